@@ -103,7 +103,7 @@ def _quant4_plain(w, group):
     padded[:, :k] = w
     v = padded.view(n, groups, group)
     top = v.abs().amax(dim=2)
-    scales = torch.where(top > 0, top / 7.0, torch.ones_like(top))
+    scales = torch.where(top > 0, top / torch.full_like(top, 7.0), torch.ones_like(top))  # by a tensor: IEEE division
     t = (v * (1.0 / scales)[:, :, None]).double()  # 64 bits: the halves are a border
     codes = (torch.sign(t) * torch.floor(t.abs() + 0.5)).clamp(-8, 7).to(torch.int8)
     return codes.view(n, groups * group)[:, :k].contiguous(), scales
