@@ -53,6 +53,7 @@ typedef enum nne_status {
 
 typedef struct nne_ctx nne_ctx;         /* one per device: streams, staging, SM count   */
 typedef struct nne_qlinear nne_qlinear; /* one device-resident int8 layer               */
+typedef struct nne_qlinear4 nne_qlinear4; /* one device-resident 4-bit layer            */
 typedef struct nne_plan nne_plan;       /* a fixed list of forwards run as one launch   */
 typedef struct nne_shard_group nne_shard_group; /* one rank's end of a column-shard exchange */
 
@@ -295,6 +296,52 @@ typedef struct nne_plan_item {
 } nne_plan_item;
 NNE_API int nne_qlinear_plan_create_fused(nne_ctx *ctx, size_t count, const nne_plan_item *items,
                                           size_t m, nne_plan **out);
+
+/* ---- 4-bit layer ----------------------------------------------------------------------------
+ * QLinear with half the weight bytes: codes of 4 bits, one f32 scale for each `group` (32, 64 or 128)
+ * consecutive inputs of a row; the last group of a row may be shorter.  The rounding rule is the one
+ * of the int8 layer (src/nn/quantized.rs:107-127) with 7 in the place of 127 and a group in the place
+ * of a row: scale = max|w_g| > 0 ? max|w_g| / 7 : 1, inv = 1 / scale, q = round_half_away(w * inv)
+ * clamped to [-8, 7], NaN -> 0.  Public layout of the codes: [n, (k + 1) / 2] bytes, two's complement,
+ * the even column in the low four bits (an odd k leaves the last high half 0); of the scales:
+ * [n, ceil(k / group)].  No counterpart in the reference.
+ *
+ * A forward computes y[r,j] = sum_g scale[j,g] * sum_{i in g} q[j,i] * x[r,i] (+ bias[j]) with the
+ * accuracy of f32: an activation enters as the sum of two 11-bit numbers (2^-22 of its group's largest
+ * |x|), products are exact, sums are f32.  A row's result does not depend on which other rows are in
+ * the batch as long as the batch stays in one of the ranges 1..4, 5..8, 9..16, 17..32.  A row of x that
+ * holds Inf or NaN gives NaN or Inf in every channel whose codes meet it; other rows are untouched.
+ * One launch, no workspace.  Weights are read once for up to 32 rows, once more for each further 32.
+ * The handle is immutable and forwards may run concurrently, as with nne_qlinear.  Limits: 2^22 rows,
+ * 2^30 columns. */
+NNE_API int nne_quantize_rows4_dev(nne_ctx *ctx, const float *w_dev, size_t rows, size_t cols, size_t group,
+                                   uint8_t *q_dev, float *scales_dev, void *stream);
+NNE_API int nne_qlinear4_create_from_f32(nne_ctx *ctx, const float *w_host, const float *bias_host_or_null,
+                                         size_t n, size_t k, size_t group, nne_qlinear4 **out);
+NNE_API int nne_qlinear4_create_from_f32_dev(nne_ctx *ctx, const float *w_dev, const float *bias_dev_or_null,
+                                             size_t n, size_t k, size_t group, void *stream, nne_qlinear4 **out);
+/* From codes and scales in the public layout; the buffers are not kept.  The _dev forms of creation
+ * wait for `stream`: the layer is complete when they return. */
+NNE_API int nne_qlinear4_create_from_i4(nne_ctx *ctx, const uint8_t *q_host, const float *scales_host,
+                                        const float *bias_host_or_null, size_t n, size_t k, size_t group,
+                                        nne_qlinear4 **out);
+NNE_API int nne_qlinear4_create_from_i4_dev(nne_ctx *ctx, const uint8_t *q_dev, const float *scales_dev,
+                                            const float *bias_dev_or_null, size_t n, size_t k, size_t group,
+                                            void *stream, nne_qlinear4 **out);
+NNE_API int nne_qlinear4_destroy(nne_qlinear4 *ql);
+/* Codes and scales in the public layout; either pointer may be NULL. */
+NNE_API int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host);
+/* The f32 weights [n, k] the layer stands for, q * scale (as QLinear::to_linear, src/nn/quantized.rs:200-209). */
+NNE_API int nne_qlinear4_dequantize(const nne_qlinear4 *ql, float *w_host);
+NNE_API int nne_qlinear4_info(const nne_qlinear4 *ql, size_t *n, size_t *k, size_t *group, int *has_bias);
+/* Device bytes of the layer: codes and scales padded to 16 rows and 64 columns, and the bias. */
+NNE_API size_t nne_qlinear4_memory_bytes(const nne_qlinear4 *ql);
+/* The three forwards of nne_qlinear, with the same checks. */
+NNE_API int nne_qlinear4_forward_host(nne_qlinear4 *ql, const float *x_host, size_t m, size_t k, float *y_host);
+NNE_API int nne_qlinear4_forward_dev(nne_qlinear4 *ql, const float *x_dev, size_t m, size_t k, float *y_dev,
+                                     void *stream);
+NNE_API int nne_qlinear4_forward_dev_strided(nne_qlinear4 *ql, const float *x_dev, size_t m, size_t k,
+                                             float *y_dev, size_t ldy, void *stream);
 
 /* ---- column shards over the GPUs of one node -------------------------------------------------
  * The reference has no multi-device code.  Its forward computes output channel j from row j of

@@ -79,6 +79,26 @@ SIGNATURES = {
     "nne_silu_mul_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
     "nne_add_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
     "nne_qlinear_plan_create_fused": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, c_void_pp]),
+    "nne_quantize_rows4_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p,
+                                         C.c_void_p, C.c_void_p]),
+    "nne_qlinear4_create_from_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t,
+                                               c_void_pp]),
+    "nne_qlinear4_create_from_f32_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t,
+                                                   C.c_size_t, C.c_void_p, c_void_pp]),
+    "nne_qlinear4_create_from_i4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t,
+                                              C.c_size_t, c_void_pp]),
+    "nne_qlinear4_create_from_i4_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                                  C.c_size_t, C.c_size_t, C.c_void_p, c_void_pp]),
+    "nne_qlinear4_destroy": (C.c_int, [C.c_void_p]),
+    "nne_qlinear4_download": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nne_qlinear4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nne_qlinear4_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t),
+                                    C.POINTER(C.c_int)]),
+    "nne_qlinear4_memory_bytes": (C.c_size_t, [C.c_void_p]),
+    "nne_qlinear4_forward_host": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p]),
+    "nne_qlinear4_forward_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "nne_qlinear4_forward_dev_strided": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                                   C.c_size_t, C.c_void_p]),
     "nne_shard_group_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, c_void_pp]),
     "nne_shard_group_handle": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nne_shard_group_connect": (C.c_int, [C.c_void_p, C.c_void_p]),

@@ -1,0 +1,850 @@
+// Linear layer with 4-bit weights and one f32 scale per group of 32, 64 or 128 consecutive inputs:
+//
+//   scale[j,g] = max|w_g| > 0 ? max|w_g| / 7 : 1,   q = clamp(round_half_away(w * (1/scale)), -8, 7)
+//   y[r,j]     = sum_g scale[j,g] * sum_{i in g} q[j,i] * x[r,i]   (+ bias[j])
+//
+// the rounding rule of Int8Tensor / QLinear (src/nn/quantized.rs:107-127) with 7 in the place of 127 and a
+// scale per group in the place of one per row.
+//
+// Public layout: codes [n, ceil(k/2)] bytes, two's complement, the even column in the low four bits; scales
+// [n, ceil(k/group)].  On the device the layer keeps one private copy, laid out for the forward kernel: tiles of
+// 16 rows x 64 columns, 512 bytes each, in which lane l's 16 bytes hold its operand fragments of four
+// m16n8k16 MMAs (a code as q + 8, so that three integer operations turn four codes into two f16 pairs), and the
+// scales as [tile][group][8][2] (rows r and r + 8 side by side: what one lane needs).  k is padded to 64 and n to
+// 16 with zero codes.
+#include <cuda_fp16.h>
+
+#include <new>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+struct nne_qlinear4 {
+    nne_ctx *ctx = nullptr;
+    int device = 0;
+    size_t n = 0, k = 0;
+    int group = 0;
+    size_t tiles = 0, chunks = 0, groups = 0;  // ceil(n/16), ceil(k/64), ceil(k/group)
+    uint4 *words = nullptr;                    // [tiles][chunks][32]
+    float2 *scales = nullptr;                  // [tiles][groups of the padded k][8]
+    float *bias = nullptr;                     // [n] or null
+};
+
+namespace nne {
+namespace {
+
+constexpr int Q4_ROWS = 16;        // rows of a tile
+constexpr int Q4_CHUNK = 64;       // columns of a tile
+constexpr int Q4_WARPS = 8;        // row tiles (one a warp) of a CTA
+constexpr int Q4_MAX_SPLIT = 8;    // CTAs of a cluster that share a row block's columns
+
+__host__ __device__ inline size_t padded_groups(size_t chunks, int group) {
+    return group >= Q4_CHUNK ? (chunks * Q4_CHUNK + group - 1) / group : chunks * (Q4_CHUNK / group);
+}
+
+// ---- quantize ---------------------------------------------------------------------------------------------
+// A thread takes eight consecutive columns, a warp 256; a group is 4, 8 or 16 lanes, whose maximum is found by
+// shuffles, so a matrix is read once.  HBM bound: 4 bytes in and half a byte out per weight.
+__device__ __forceinline__ int code4(float v, float inv) {
+    const float t = __fmul_rn(v, inv);
+    if (!(t == t)) return 0;  // NaN
+    const float r = roundf(t);  // halves away from zero
+    return (int)fminf(fmaxf(r, -8.0f), 7.0f);
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(256)
+quantize_rows4_kernel(const float *__restrict__ w, size_t rows, size_t cols, int group, uint8_t *__restrict__ q,
+                      float *__restrict__ scales) {
+    const int lane = threadIdx.x & 31;
+    const size_t segs = (cols + 255) / 256, bytes = (cols + 1) / 2, groups = (cols + group - 1) / group;
+    const size_t total = rows * segs, step = (size_t)gridDim.x * 8;
+    const int width = group / 8;  // lanes of a group
+    for (size_t it = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < total; it += step) {
+        const size_t r = it / segs, c = (it - r * segs) * 256 + lane * 8;
+        const float *p = w + r * cols + c;
+        float v[8];
+        if (VEC) {  // cols % 8 == 0: a lane's columns are all there or all behind the row
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 f = c < cols ? __ldcs(reinterpret_cast<const float4 *>(p) + h) : make_float4(0, 0, 0, 0);
+                v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? p[i] : 0.0f;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));  // NaN is passed over
+        for (int o = 1; o < width; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float scale = top > 0.0f ? __fdiv_rn(top, 7.0f) : 1.0f;
+        const float inv = __fdiv_rn(1.0f, scale);
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= (uint32_t)(code4(v[i], inv) & 15) << (4 * i);
+        if (c >= cols) continue;  // after the shuffles
+        if (lane % width == 0) scales[r * groups + c / group] = scale;
+        uint8_t *o = q + r * bytes + c / 2;
+        if (VEC) {
+            *reinterpret_cast<uint32_t *>(o) = word;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + 2 * i < cols) o[i] = (uint8_t)(word >> (8 * i));  // codes behind the row are 0
+        }
+    }
+}
+
+// Column (within a 16 x 16 step) and row of a lane's code `i` of a fragment word: bits 4i..4i+3.  The order makes
+// (w & 0x000f000f) the pair of A register 0, (w & 0x00f000f0) that of register 1, and the same of w >> 8 those of
+// registers 2 and 3.
+__host__ __device__ inline void code_place(int lane, int i, int *row, int *col) {
+    const int g = lane >> 2, t = lane & 3;
+    const int reg = (i & 1) + ((i & 2) ? 2 : 0), high = i >> 2;
+    *row = g + ((reg & 1) ? 8 : 0);
+    *col = 2 * t + ((reg & 2) ? 8 : 0) + high;
+}
+
+// Public layout -> the forward's (one thread a 16-byte lane item), and back (one thread a byte).
+__global__ void __launch_bounds__(256)
+pack_words_kernel(const uint8_t *__restrict__ q, size_t n, size_t k, size_t chunks, size_t total, uint4 *__restrict__ words) {
+    const size_t bytes = (k + 1) / 2;
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (size_t)gridDim.x * 256) {
+        const int lane = (int)(it & 31);
+        const size_t tc = it >> 5, tile = tc / chunks, chunk = tc - tile * chunks;
+        uint32_t out[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            out[s] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                int row, col;
+                code_place(lane, i, &row, &col);
+                const size_t r = tile * Q4_ROWS + row, c = chunk * Q4_CHUNK + s * 16 + col;
+                uint32_t code = 0;
+                if (r < n && c < k) code = (q[r * bytes + c / 2] >> (4 * (c & 1))) & 15u;
+                out[s] |= (code ^ 8u) << (4 * i);  // two's complement -> q + 8
+            }
+        }
+        words[it] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+}
+__global__ void __launch_bounds__(256)
+pack_scales_kernel(const float *__restrict__ s, size_t n, size_t groups, size_t pgroups, size_t total, float2 *__restrict__ out) {
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (size_t)gridDim.x * 256) {
+        const size_t g8 = it & 7, tg = it >> 3, tile = tg / pgroups, grp = tg - tile * pgroups;
+        const size_t r = tile * Q4_ROWS + g8;
+        float2 v = make_float2(0.0f, 0.0f);  // rows and groups behind the matrix add nothing
+        if (grp < groups) {
+            if (r < n) v.x = s[r * groups + grp];
+            if (r + 8 < n) v.y = s[(r + 8) * groups + grp];
+        }
+        out[it] = v;
+    }
+}
+
+__device__ __forceinline__ int code_at(const uint4 *words, size_t chunks, size_t r, size_t c) {
+    const size_t tile = r / Q4_ROWS, chunk = c / Q4_CHUNK;
+    const int row = (int)(r % Q4_ROWS), step = (int)(c % Q4_CHUNK) / 16, col = (int)(c % 16);
+    const int reg = (row >= 8 ? 1 : 0) + (col >= 8 ? 2 : 0);
+    const int lane = (row & 7) * 4 + (col & 7) / 2, i = reg + 4 * (col & 1);
+    const uint32_t w = reinterpret_cast<const uint32_t *>(words)[((tile * chunks + chunk) * 32 + lane) * 4 + step];
+    return (int)((w >> (4 * i)) & 15u) - 8;
+}
+__global__ void __launch_bounds__(256)
+unpack_codes_kernel(const uint4 *__restrict__ words, size_t n, size_t k, size_t chunks, uint8_t *__restrict__ q) {
+    const size_t bytes = (k + 1) / 2, total = n * bytes;
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < total; it += (size_t)gridDim.x * 256) {
+        const size_t r = it / bytes, c = (it - r * bytes) * 2;
+        int v = code_at(words, chunks, r, c) & 15;
+        if (c + 1 < k) v |= (code_at(words, chunks, r, c + 1) & 15) << 4;
+        q[it] = (uint8_t)v;
+    }
+}
+__global__ void __launch_bounds__(256)
+unpack_scales_kernel(const float2 *__restrict__ s, size_t n, size_t groups, size_t pgroups, float *__restrict__ out) {
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < n * groups; it += (size_t)gridDim.x * 256) {
+        const size_t r = it / groups, grp = it - r * groups;
+        const float2 v = s[((r / Q4_ROWS) * pgroups + grp) * 8 + (r & 7)];
+        out[it] = (r & 8) ? v.y : v.x;
+    }
+}
+// w = q * scale, one product, like QLinear::to_linear (src/nn/quantized.rs:200-209)
+__global__ void __launch_bounds__(256)
+dequantize4_kernel(const uint4 *__restrict__ words, const float2 *__restrict__ s, size_t n, size_t k, size_t chunks, int group,
+                   size_t pgroups, float *__restrict__ out) {
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < n * k; it += (size_t)gridDim.x * 256) {
+        const size_t r = it / k, c = it - r * k;
+        const float2 v = s[((r / Q4_ROWS) * pgroups + c / group) * 8 + (r & 7)];
+        out[it] = __fmul_rn((float)code_at(words, chunks, r, c), (r & 8) ? v.y : v.x);
+    }
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------
+// The weights are the 16-row side of mma.sync m16n8k16 (f16, exact: a code is an integer), the activations the
+// 8-column side.  An activation is the sum of two f16 numbers (columns 2r and 2r + 1 of a step: its rounding to
+// f16, and what that leaves), 22 bits, after a power of two that brings the largest |x| of its group of columns
+// to [2^13, 2^14): the product keeps f32's accuracy, where one f16 would give 2^-11.  Products are exact, sums are f32;
+// at a group's end the two columns are added and go into the row's sum with scale * 2^-e.
+//
+// A CTA takes 128 rows (a tile a warp) and a share of the columns; the CTAs of a cluster take the shares of one
+// row block and add their sums up through each other's shared memory in rank order, so results do not change from
+// run to run, and no workspace is needed.  Each warp streams its weights straight into registers, Q4_DEPTH loads of
+// 512 bytes ahead, and they start before the wait for the kernel that makes x (a layer never changes).
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight codes of a word as the four A registers of a step.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&a)[4]) {
+    const uint32_t h = w >> 8;
+    const uint32_t magic = 0x64006400u;  // 1024 + code, or 1024 + 16 * code
+    const __half2 off = __half2half2(__ushort_as_half(0xe408));    // -1032 = -(1024 + 8)
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+    const __half2 off16 = __half2half2(__ushort_as_half(0xd480));  // -72 = -(1024 / 16 + 8)
+    uint32_t u[4] = {(w & 0x000f000fu) | magic, (w & 0x00f000f0u) | magic, (h & 0x000f000fu) | magic, (h & 0x00f000f0u) | magic};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __half2 v = *reinterpret_cast<__half2 *>(&u[i]);
+        v = (i & 1) ? __hfma2(v, sixteenth, off16) : __hadd2(v, off);
+        a[i] = *reinterpret_cast<uint32_t *>(&v);
+    }
+}
+
+struct Q4Args {
+    const uint4 *words;
+    const float2 *scales;
+    const float *bias, *x;
+    float *y;
+    size_t n, k, m, ldy;
+    unsigned tiles, chunks, pgroups;
+    unsigned span;    // chunks of a CTA's share
+    unsigned stage;   // chunks whose activations are in shared memory at once
+    int vec;          // rows of x can be read as float4
+};
+
+template <int NT>
+struct Q4Shape {
+    static constexpr int COLS = 4 * NT;                  // activation rows of a CTA
+    static constexpr int DEPTH = NT >= 8 ? 4 : 8;        // weight loads in flight a lane
+    static constexpr int CHUNK_BYTES = 4 * NT * 256;     // fragments of 64 columns
+};
+
+template <int GROUP, int NT>
+__global__ void __launch_bounds__(Q4_WARPS * 32, 2) q4_forward_kernel(const Q4Args p) {
+    using S = Q4Shape<NT>;
+    constexpr int GPC = GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP;   // scale pairs a chunk needs
+    constexpr int CPG = GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1;   // chunks of a group
+    constexpr int STEPS = GROUP >= Q4_CHUNK ? 4 : GROUP / 16;       // MMA steps between two group ends
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint2 *frag = reinterpret_cast<uint2 *>(smem);                                       // [chunk][4][NT][32]
+    float *factor = reinterpret_cast<float *>(smem + (size_t)p.stage * S::CHUNK_BYTES);  // [group][COLS]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned split = gridDim.x, rank = blockIdx.x;
+    const unsigned tile = blockIdx.y * Q4_WARPS + warp;
+    const size_t row0 = (size_t)blockIdx.z * S::COLS;  // first activation row
+    const int cols = (int)(p.m - row0 < (size_t)S::COLS ? p.m - row0 : S::COLS);
+    const unsigned c_begin = rank * p.span < p.chunks ? rank * p.span : p.chunks;
+    const unsigned c_end = c_begin + p.span < p.chunks ? c_begin + p.span : p.chunks;
+    const bool mine = tile < p.tiles;
+
+    const uint4 *wp = p.words + ((size_t)(mine ? tile : 0) * p.chunks) * 32 + lane;
+    const float2 *sp = p.scales + (size_t)(mine ? tile : 0) * p.pgroups * 8 + (lane >> 2);
+    uint4 ring[S::DEPTH];
+    float2 sring[S::DEPTH][GPC];
+    auto fetch = [&](unsigned c, uint4 &w, float2 (&s)[GPC]) {
+        if (mine && c < c_end) {
+            w = __ldcs(wp + (size_t)c * 32);
+#pragma unroll
+            for (int g = 0; g < GPC; ++g) s[g] = __ldg(sp + ((size_t)(c / CPG) * GPC + g) * 8);
+        } else {
+            w = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int g = 0; g < GPC; ++g) s[g] = make_float2(0.0f, 0.0f);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < S::DEPTH; ++j) fetch(c_begin + j, ring[j], sring[j]);
+
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    float sum[NT][2], part[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        sum[t][0] = sum[t][1] = 0.0f;
+        part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.0f;
+    }
+
+    for (unsigned s0 = c_begin; s0 < c_end; s0 += p.stage) {
+        const unsigned s1 = s0 + p.stage < c_end ? s0 + p.stage : c_end;
+        // Activations of these chunks: a warp takes 128 columns of one row at a time, four a lane.
+        if (s0 != c_begin) __syncthreads();
+        const unsigned blocks = (s1 - s0 + 1) / 2;
+        for (unsigned b = warp; b < blocks * S::COLS; b += Q4_WARPS) {
+            const unsigned r = b % S::COLS, blk = b / S::COLS;
+            const unsigned ck = s0 + 2 * blk + (lane >> 4);  // this lane's chunk
+            const size_t c = (size_t)ck * Q4_CHUNK + (lane & 15) * 4;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if ((int)r < cols && ck < s1) {
+                const float *src = p.x + (row0 + r) * p.k + c;
+                if (p.vec) {
+                    if (c < p.k) {
+                        const float4 f = *reinterpret_cast<const float4 *>(src);
+                        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < p.k) v[i] = src[i];
+                }
+            }
+            float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+            for (int o = 1; o < GROUP / 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // 2^e by its bits: top * 2^e in [2^13, 2^14); e within -114 .. 126 keeps 2^e and 2^-e normal
+            const int be = (int)(__float_as_uint(top) >> 23) & 255;
+            int e = 13 + 127 - be;
+            e = e > 126 ? 126 : (e < -114 ? -114 : e);
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+            if (ck < s1) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float a = v[2 * h] * up, d = v[2 * h + 1] * up;
+                    const __half2 hh = __floats2half2_rn(a, d);
+                    const float2 back = __half22float2(hh);
+                    const __half2 ll = __floats2half2_rn(a - back.x, d - back.y);
+                    hi[h] = *reinterpret_cast<const uint32_t *>(&hh);
+                    lo[h] = *reinterpret_cast<const uint32_t *>(&ll);
+                }
+                const int kk = (lane & 3) * 4, step = (lane & 15) >> 2;
+                const int t = (kk & 7) / 2, word = kk >> 3, g = 2 * (r & 3);
+                uint32_t *f = reinterpret_cast<uint32_t *>(frag + (((size_t)(ck - s0) * 4 + step) * NT + r / 4) * 32);
+                f[(g * 4 + t) * 2 + word] = hi[0];
+                f[(g * 4 + t + 1) * 2 + word] = hi[1];
+                f[((g + 1) * 4 + t) * 2 + word] = lo[0];
+                f[((g + 1) * 4 + t + 1) * 2 + word] = lo[1];
+                if ((lane * 4) % GROUP == 0) {
+                    const unsigned grp = GROUP >= Q4_CHUNK ? (ck - s0) / CPG : (ck - s0) * GPC + ((lane & 15) * 4) / GROUP;
+                    factor[(size_t)grp * S::COLS + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+                }
+            }
+        }
+        __syncthreads();
+
+        for (unsigned base = s0; base < s1; base += S::DEPTH) {
+#pragma unroll
+            for (int j = 0; j < S::DEPTH; ++j) {
+                const unsigned c = base + j;
+                if (c < s1) {  // the same for the whole CTA
+                    const uint4 w4 = ring[j];
+                    float2 sc[GPC];
+#pragma unroll
+                    for (int g = 0; g < GPC; ++g) sc[g] = sring[j][g];
+                    fetch(c + S::DEPTH, ring[j], sring[j]);
+                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    const uint2 *fc = frag + (size_t)(c - s0) * 4 * NT * 32 + lane;
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        uint32_t a[4];
+                        codes_to_f16(w[st], a);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            const uint2 b = fc[(st * NT + t) * 32];
+                            mma_f16(part[t], a, b.x, b.y);
+                        }
+                        if (st % STEPS == STEPS - 1 && (CPG == 1 || ((c - s0) % CPG) == CPG - 1 || c + 1 == c_end)) {
+                            const float2 s2 = sc[GPC == 1 ? 0 : st / STEPS];
+                            const unsigned grp = CPG > 1 ? (c - s0) / CPG : (c - s0) * GPC + st / STEPS;
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                const float f = factor[(size_t)grp * S::COLS + t * 4 + (lane & 3)];
+                                sum[t][0] = fmaf(s2.x * f, part[t][0] + part[t][1], sum[t][0]);
+                                sum[t][1] = fmaf(s2.y * f, part[t][2] + part[t][3], sum[t][1]);
+                                part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.0f;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // Sums of the cluster's CTAs: each leaves [128][COLS] in its shared memory, and rank i adds up every
+    // split-th row of all of them, rank after rank.
+    float *mysum = reinterpret_cast<float *>(smem);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        mysum[(warp * 16 + (lane >> 2)) * S::COLS + t * 4 + (lane & 3)] = sum[t][0];
+        mysum[(warp * 16 + (lane >> 2) + 8) * S::COLS + t * 4 + (lane & 3)] = sum[t][1];
+    }
+    if (split > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    const size_t out0 = (size_t)blockIdx.y * (Q4_WARPS * Q4_ROWS);
+    const unsigned per = (Q4_WARPS * Q4_ROWS + split - 1) / split;  // rows of this rank
+    for (unsigned i = threadIdx.x; i < per * S::COLS; i += Q4_WARPS * 32) {
+        // neighbouring threads take neighbouring rows: y is written in runs along n
+        const unsigned r = rank * per + i % per, c = i / per;
+        if (r >= Q4_WARPS * Q4_ROWS || out0 + r >= p.n || (int)c >= cols) continue;
+        float v = 0.0f;
+        const uint32_t at = smem_u32(mysum + r * S::COLS + c);
+        for (unsigned q = 0; q < split; ++q) {
+            float u;
+            uint32_t peer;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(q));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(peer) : "memory");
+            v += u;
+        }
+        if (p.bias) v = __fadd_rn(v, p.bias[out0 + r]);
+        p.y[(row0 + c) * p.ldy + out0 + r] = v;
+    }
+    if (split > 1)  // nobody leaves while a peer may still read its shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int GROUP, int NT>
+int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
+    using S = Q4Shape<NT>;
+    const nne_ctx *ctx = ql->ctx;
+    const size_t blocks_n = (ql->tiles + Q4_WARPS - 1) / Q4_WARPS;
+    const size_t blocks_m = (m + S::COLS - 1) / S::COLS;
+    if (blocks_n > 65535 || blocks_m > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "layer or batch too large for one launch");
+    // Split the columns until two CTAs an SM are there, as long as a share keeps four chunks of 64.
+    const size_t want = 2 * (size_t)ctx->sm_count, have = blocks_n * blocks_m;
+    unsigned split = (unsigned)((want + have - 1) / have);
+    if (split > Q4_MAX_SPLIT) split = Q4_MAX_SPLIT;
+    while (split > 1 && ql->chunks < (size_t)split * 4) --split;
+    // shares in whole pairs of chunks, so that a group of 128 columns never lies in two
+    size_t span = (ql->chunks + split - 1) / split;
+    span = (span + 1) & ~(size_t)1;
+    split = (unsigned)((ql->chunks + span - 1) / span);
+    // activations staged at once: at most 96 KB, so that two CTAs fit an SM
+    size_t stage = (size_t)98304 / (S::CHUNK_BYTES + 2 * S::COLS * sizeof(float));
+    stage = stage & ~(size_t)7;  // whole rounds of the register ring
+    if (stage > span) stage = span;
+    Q4Args a = {};
+    a.words = ql->words;
+    a.scales = ql->scales;
+    a.bias = ql->bias;
+    a.x = x;
+    a.y = y;
+    a.n = ql->n;
+    a.k = ql->k;
+    a.m = m;
+    a.ldy = ldy;
+    a.tiles = (unsigned)ql->tiles;
+    a.chunks = (unsigned)ql->chunks;
+    a.pgroups = (unsigned)padded_groups(ql->chunks, GROUP);
+    a.span = (unsigned)span;
+    a.stage = (unsigned)stage;
+    a.vec = ql->k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    size_t bytes = stage * S::CHUNK_BYTES + (stage * Q4_CHUNK / GROUP + 1) * S::COLS * sizeof(float);
+    const size_t sums = (size_t)Q4_WARPS * Q4_ROWS * S::COLS * sizeof(float);
+    if (bytes < sums) bytes = sums;
+    NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT>, bytes));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, (unsigned)blocks_n, (unsigned)blocks_m);
+    cfg.blockDim = dim3(Q4_WARPS * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = split;
+    attr[na].val.clusterDim.y = 1;
+    attr[na].val.clusterDim.z = 1;
+    ++na;
+    if (pdl_enabled()) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_forward_kernel<GROUP, NT>, a);
+    count_launch();
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(NNE_ERR_CUDA, "4-bit forward launch failed: %s", cudaGetErrorString(e));
+    }
+    return NNE_OK;
+}
+
+template <int GROUP>
+int launch_q4_group(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
+    if (m <= 4) return launch_q4<GROUP, 1>(ql, x, m, y, ldy, s);
+    if (m <= 8) return launch_q4<GROUP, 2>(ql, x, m, y, ldy, s);
+    if (m <= 16) return launch_q4<GROUP, 4>(ql, x, m, y, ldy, s);
+    return launch_q4<GROUP, 8>(ql, x, m, y, ldy, s);
+}
+
+__global__ void __launch_bounds__(256)
+fill_bias_kernel(const float *__restrict__ bias, size_t n, size_t m, size_t ldy, float *__restrict__ y) {
+    for (size_t it = (size_t)blockIdx.x * 256 + threadIdx.x; it < n * m; it += (size_t)gridDim.x * 256)
+        y[(it / n) * ldy + it % n] = bias ? bias[it % n] : 0.0f;
+}
+
+unsigned grid_of(const nne_ctx *ctx, size_t items, size_t per_block) {
+    size_t b = (items + per_block - 1) / per_block;
+    const size_t cap = (size_t)ctx->sm_count * 8;
+    return (unsigned)(b < 1 ? 1 : (b > cap ? cap : b));
+}
+
+int launch_quantize4(nne_ctx *ctx, const float *w, size_t rows, size_t cols, int group, uint8_t *q, float *scales, cudaStream_t s) {
+    if (rows == 0 || cols == 0) return NNE_OK;
+    const unsigned grid = grid_of(ctx, rows * ((cols + 255) / 256), 8);
+    const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
+    if (vec)
+        quantize_rows4_kernel<true><<<grid, 256, 0, s>>>(w, rows, cols, group, q, scales);
+    else
+        quantize_rows4_kernel<false><<<grid, 256, 0, s>>>(w, rows, cols, group, q, scales);
+    NNE_LAUNCH_CHECK();
+    return NNE_OK;
+}
+
+int check_group(size_t group) {
+    if (group != 32 && group != 64 && group != 128)
+        return fail(NNE_ERR_INVALID_ARGUMENT, "group must be 32, 64 or 128 columns, got %zu", group);
+    return NNE_OK;
+}
+
+// Sizes whose byte counts fit size_t, and tile counts that fit the kernels' 32-bit ones.
+int check_sizes(size_t n, size_t k) {
+    size_t t;
+    if (__builtin_mul_overflow(n, k, &t) || __builtin_mul_overflow(t, sizeof(float), &t))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "n*k overflows size_t");
+    if (n > ((size_t)1 << 22) || k > ((size_t)1 << 30))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "a 4-bit layer holds at most 2^22 rows of 2^30 columns, got %zu x %zu", n, k);
+    return NNE_OK;
+}
+
+int alloc_layer4(nne_ctx *ctx, size_t n, size_t k, size_t group, bool has_bias, nne_qlinear4 **out) {
+    NNE_TRY(check_group(group));
+    NNE_TRY(check_sizes(n, k));
+    nne_qlinear4 *ql = new (std::nothrow) nne_qlinear4();
+    if (!ql) return fail(NNE_ERR_OUT_OF_MEMORY, "host allocation failed");
+    ql->ctx = ctx;
+    ql->device = ctx->device;
+    ql->n = n;
+    ql->k = k;
+    ql->group = (int)group;
+    ql->tiles = (n + Q4_ROWS - 1) / Q4_ROWS;
+    ql->chunks = (k + Q4_CHUNK - 1) / Q4_CHUNK;
+    ql->groups = (k + group - 1) / group;
+    const size_t wb = ql->tiles * ql->chunks * 32 * sizeof(uint4);
+    const size_t sb = ql->tiles * padded_groups(ql->chunks, ql->group) * 8 * sizeof(float2);
+    cudaError_t e = cudaMalloc(&ql->words, wb ? wb : 16);
+    if (e == cudaSuccess) e = cudaMalloc(&ql->scales, sb ? sb : 16);
+    if (e == cudaSuccess && has_bias) e = cudaMalloc(&ql->bias, (n ? n : 1) * sizeof(float));
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        const int st = fail(e == cudaErrorMemoryAllocation ? NNE_ERR_OUT_OF_MEMORY : NNE_ERR_CUDA,
+                            "device allocation for a %zu x %zu 4-bit layer failed: %s", n, k, cudaGetErrorString(e));
+        nne_qlinear4_destroy(ql);
+        return st;
+    }
+    *out = ql;
+    return NNE_OK;
+}
+
+// Fills a layer from codes and scales in the public layout (device pointers) and waits for it: the layer is handed
+// out complete, since forwards read the weights ahead of the stream's earlier work.
+int fill_layer4(nne_qlinear4 *ql, const uint8_t *q, const float *scales, const float *bias, cudaMemcpyKind bias_from, cudaStream_t s) {
+    const size_t pg = padded_groups(ql->chunks, ql->group);
+    const size_t words = ql->tiles * ql->chunks * 32, pairs = ql->tiles * pg * 8;
+    if (words) {
+        pack_words_kernel<<<grid_of(ql->ctx, words, 256), 256, 0, s>>>(q, ql->n, ql->k, ql->chunks, words, ql->words);
+        NNE_LAUNCH_CHECK();
+        pack_scales_kernel<<<grid_of(ql->ctx, pairs, 256), 256, 0, s>>>(scales, ql->n, ql->groups, pg, pairs, ql->scales);
+        NNE_LAUNCH_CHECK();
+    }
+    if (bias && ql->n) NNE_CUDA_TRY(cudaMemcpyAsync(ql->bias, bias, ql->n * sizeof(float), bias_from, s));
+    NNE_CUDA_TRY(cudaStreamSynchronize(s));
+    return NNE_OK;
+}
+
+int forward4(nne_qlinear4 *ql, const float *x, size_t m, size_t k, float *y, size_t ldy, cudaStream_t s) {
+    if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
+    if (k != ql->k) return fail(NNE_ERR_SHAPE_MISMATCH, "shape mismatch: expected [%zu], got [%zu]", ql->k, k);
+    if (ldy < ql->n) return fail(NNE_ERR_INVALID_ARGUMENT, "ldy %zu < out_features %zu", ldy, ql->n);
+    size_t t;
+    if (__builtin_mul_overflow(m, ql->k, &t) || __builtin_mul_overflow(m, ldy, &t) || __builtin_mul_overflow(t, sizeof(float), &t))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "m*k or m*ldy overflows size_t");
+    if (m == 0 || ql->n == 0) return NNE_OK;
+    if (!y || (ql->k && !x)) return fail(NNE_ERR_INVALID_ARGUMENT, "null activation or output pointer");
+    if ((reinterpret_cast<uintptr_t>(x) & 3) || (reinterpret_cast<uintptr_t>(y) & 3))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "activation or output pointer is not 4-byte aligned");
+    NNE_TRY(use_ctx(ql->ctx));
+    if (ql->k == 0) {  // an empty contraction
+        fill_bias_kernel<<<grid_of(ql->ctx, ql->n * m, 256), 256, 0, s>>>(ql->bias, ql->n, m, ldy, y);
+        NNE_LAUNCH_CHECK();
+        return NNE_OK;
+    }
+    switch (ql->group) {
+        case 32: return launch_q4_group<32>(ql, x, m, y, ldy, s);
+        case 64: return launch_q4_group<64>(ql, x, m, y, ldy, s);
+        default: return launch_q4_group<128>(ql, x, m, y, ldy, s);
+    }
+}
+
+// A stream-ordered device buffer for the length of a creation or download.
+struct Scratch {
+    void *p = nullptr;
+    cudaStream_t s;
+    explicit Scratch(cudaStream_t stream) : s(stream) {}
+    int get(size_t bytes) {
+        NNE_CUDA_TRY(cudaMallocAsync(&p, bytes ? bytes : 16, s));
+        return NNE_OK;
+    }
+    ~Scratch() {
+        if (p) cudaFreeAsync(p, s);
+    }
+};
+
+// Quantizes device weights into `ql`.
+int quantize_into4(nne_qlinear4 *ql, const float *w_dev, const float *bias, cudaMemcpyKind bias_from, cudaStream_t s) {
+    Scratch q(s), sc(s);
+    NNE_TRY(q.get(ql->n * ((ql->k + 1) / 2)));
+    NNE_TRY(sc.get(ql->n * ql->groups * sizeof(float)));
+    NNE_TRY(launch_quantize4(ql->ctx, w_dev, ql->n, ql->k, ql->group, (uint8_t *)q.p, (float *)sc.p, s));
+    return fill_layer4(ql, (const uint8_t *)q.p, (const float *)sc.p, bias, bias_from, s);
+}
+
+}  // namespace
+}  // namespace nne
+
+using namespace nne;
+
+extern "C" {
+
+int nne_quantize_rows4_dev(nne_ctx *ctx, const float *w_dev, size_t rows, size_t cols, size_t group, uint8_t *q_dev,
+                           float *scales_dev, void *stream) {
+    NNE_GUARD_BEGIN
+    NNE_TRY(use_ctx(ctx));
+    NNE_TRY(check_group(group));
+    size_t t;
+    if (__builtin_mul_overflow(rows, cols, &t) || __builtin_mul_overflow(t, sizeof(float), &t))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "rows*cols overflows size_t");
+    if (rows == 0 || cols == 0) return NNE_OK;
+    if (!w_dev || !q_dev || !scales_dev) return fail(NNE_ERR_INVALID_ARGUMENT, "null device pointer");
+    return launch_quantize4(ctx, w_dev, rows, cols, (int)group, q_dev, scales_dev, (cudaStream_t)stream);
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_create_from_f32_dev(nne_ctx *ctx, const float *w_dev, const float *bias_dev_or_null, size_t n, size_t k,
+                                     size_t group, void *stream, nne_qlinear4 **out) {
+    NNE_GUARD_BEGIN
+    if (!out) return fail(NNE_ERR_INVALID_ARGUMENT, "null out pointer");
+    *out = nullptr;
+    NNE_TRY(use_ctx(ctx));
+    if (n && k && !w_dev) return fail(NNE_ERR_INVALID_ARGUMENT, "null weight pointer");
+    nne_qlinear4 *ql = nullptr;
+    NNE_TRY(alloc_layer4(ctx, n, k, group, bias_dev_or_null != nullptr, &ql));
+    const int st = quantize_into4(ql, w_dev, bias_dev_or_null, cudaMemcpyDeviceToDevice, (cudaStream_t)stream);
+    if (st != NNE_OK) {
+        nne_qlinear4_destroy(ql);
+        return st;
+    }
+    *out = ql;
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_create_from_f32(nne_ctx *ctx, const float *w_host, const float *bias_host_or_null, size_t n, size_t k,
+                                 size_t group, nne_qlinear4 **out) {
+    NNE_GUARD_BEGIN
+    if (!out) return fail(NNE_ERR_INVALID_ARGUMENT, "null out pointer");
+    *out = nullptr;
+    NNE_TRY(use_ctx(ctx));
+    if (n && k && !w_host) return fail(NNE_ERR_INVALID_ARGUMENT, "null weight pointer");
+    nne_qlinear4 *ql = nullptr;
+    NNE_TRY(alloc_layer4(ctx, n, k, group, bias_host_or_null != nullptr, &ql));
+    int st = NNE_OK;
+    {
+        std::lock_guard<std::mutex> lock(ctx->mu);
+        const size_t bytes = n * k * sizeof(float);
+        st = ctx->stage_a.reserve(bytes ? bytes : 4);
+        cudaError_t e = cudaSuccess;
+        if (st == NNE_OK && bytes) e = cudaMemcpyAsync(ctx->stage_a.ptr, w_host, bytes, cudaMemcpyHostToDevice, ctx->stream);
+        if (e != cudaSuccess) st = fail(NNE_ERR_CUDA, "layer upload failed: %s", cudaGetErrorString(e));
+        if (st == NNE_OK) st = quantize_into4(ql, (const float *)ctx->stage_a.ptr, bias_host_or_null, cudaMemcpyHostToDevice, ctx->stream);
+    }
+    if (st != NNE_OK) {
+        nne_qlinear4_destroy(ql);
+        return st;
+    }
+    *out = ql;
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_create_from_i4_dev(nne_ctx *ctx, const uint8_t *q_dev, const float *scales_dev, const float *bias_dev_or_null,
+                                    size_t n, size_t k, size_t group, void *stream, nne_qlinear4 **out) {
+    NNE_GUARD_BEGIN
+    if (!out) return fail(NNE_ERR_INVALID_ARGUMENT, "null out pointer");
+    *out = nullptr;
+    NNE_TRY(use_ctx(ctx));
+    if (n && k && (!q_dev || !scales_dev)) return fail(NNE_ERR_INVALID_ARGUMENT, "null codes or scales pointer");
+    nne_qlinear4 *ql = nullptr;
+    NNE_TRY(alloc_layer4(ctx, n, k, group, bias_dev_or_null != nullptr, &ql));
+    const int st = fill_layer4(ql, q_dev, scales_dev, bias_dev_or_null, cudaMemcpyDeviceToDevice, (cudaStream_t)stream);
+    if (st != NNE_OK) {
+        nne_qlinear4_destroy(ql);
+        return st;
+    }
+    *out = ql;
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_create_from_i4(nne_ctx *ctx, const uint8_t *q_host, const float *scales_host, const float *bias_host_or_null,
+                                size_t n, size_t k, size_t group, nne_qlinear4 **out) {
+    NNE_GUARD_BEGIN
+    if (!out) return fail(NNE_ERR_INVALID_ARGUMENT, "null out pointer");
+    *out = nullptr;
+    NNE_TRY(use_ctx(ctx));
+    if (n && k && (!q_host || !scales_host)) return fail(NNE_ERR_INVALID_ARGUMENT, "null codes or scales pointer");
+    nne_qlinear4 *ql = nullptr;
+    NNE_TRY(alloc_layer4(ctx, n, k, group, bias_host_or_null != nullptr, &ql));
+    int st = NNE_OK;
+    {
+        std::lock_guard<std::mutex> lock(ctx->mu);
+        cudaStream_t s = ctx->stream;
+        const size_t qb = n * ((k + 1) / 2), sb = n * ql->groups * sizeof(float);
+        Scratch q(s), sc(s);
+        st = q.get(qb);
+        if (st == NNE_OK) st = sc.get(sb);
+        cudaError_t e = cudaSuccess;
+        if (st == NNE_OK && qb) e = cudaMemcpyAsync(q.p, q_host, qb, cudaMemcpyHostToDevice, s);
+        if (st == NNE_OK && e == cudaSuccess && sb) e = cudaMemcpyAsync(sc.p, scales_host, sb, cudaMemcpyHostToDevice, s);
+        if (st == NNE_OK && e != cudaSuccess) st = fail(NNE_ERR_CUDA, "layer upload failed: %s", cudaGetErrorString(e));
+        if (st == NNE_OK) st = fill_layer4(ql, (const uint8_t *)q.p, (const float *)sc.p, bias_host_or_null, cudaMemcpyHostToDevice, s);
+    }
+    if (st != NNE_OK) {
+        nne_qlinear4_destroy(ql);
+        return st;
+    }
+    *out = ql;
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_destroy(nne_qlinear4 *ql) {
+    NNE_GUARD_BEGIN
+    if (!ql) return NNE_OK;
+    cudaSetDevice(ql->device);
+    if (ql->words) cudaFree(ql->words);
+    if (ql->scales) cudaFree(ql->scales);
+    if (ql->bias) cudaFree(ql->bias);
+    delete ql;
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host) {
+    NNE_GUARD_BEGIN
+    if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
+    if (ql->n == 0 || ql->k == 0) return NNE_OK;
+    NNE_TRY(use_ctx(ql->ctx));
+    std::lock_guard<std::mutex> lock(ql->ctx->mu);
+    cudaStream_t s = ql->ctx->stream;
+    const size_t qb = ql->n * ((ql->k + 1) / 2), sb = ql->n * ql->groups * sizeof(float);
+    Scratch q(s), sc(s);
+    if (q_host) {
+        NNE_TRY(q.get(qb));
+        unpack_codes_kernel<<<grid_of(ql->ctx, qb, 256), 256, 0, s>>>(ql->words, ql->n, ql->k, ql->chunks, (uint8_t *)q.p);
+        NNE_LAUNCH_CHECK();
+        NNE_CUDA_TRY(cudaMemcpyAsync(q_host, q.p, qb, cudaMemcpyDeviceToHost, s));
+    }
+    if (scales_host) {
+        NNE_TRY(sc.get(sb));
+        unpack_scales_kernel<<<grid_of(ql->ctx, ql->n * ql->groups, 256), 256, 0, s>>>(
+            ql->scales, ql->n, ql->groups, padded_groups(ql->chunks, ql->group), (float *)sc.p);
+        NNE_LAUNCH_CHECK();
+        NNE_CUDA_TRY(cudaMemcpyAsync(scales_host, sc.p, sb, cudaMemcpyDeviceToHost, s));
+    }
+    NNE_CUDA_TRY(cudaStreamSynchronize(s));
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_dequantize(const nne_qlinear4 *ql, float *w_host) {
+    NNE_GUARD_BEGIN
+    if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
+    if (ql->n == 0 || ql->k == 0) return NNE_OK;
+    if (!w_host) return fail(NNE_ERR_INVALID_ARGUMENT, "null host pointer");
+    NNE_TRY(use_ctx(ql->ctx));
+    std::lock_guard<std::mutex> lock(ql->ctx->mu);
+    cudaStream_t s = ql->ctx->stream;
+    Scratch w(s);
+    const size_t bytes = ql->n * ql->k * sizeof(float);
+    NNE_TRY(w.get(bytes));
+    dequantize4_kernel<<<grid_of(ql->ctx, ql->n * ql->k, 256), 256, 0, s>>>(ql->words, ql->scales, ql->n, ql->k, ql->chunks, ql->group,
+                                                                          padded_groups(ql->chunks, ql->group), (float *)w.p);
+    NNE_LAUNCH_CHECK();
+    NNE_CUDA_TRY(cudaMemcpyAsync(w_host, w.p, bytes, cudaMemcpyDeviceToHost, s));
+    NNE_CUDA_TRY(cudaStreamSynchronize(s));
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_info(const nne_qlinear4 *ql, size_t *n, size_t *k, size_t *group, int *has_bias) {
+    if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
+    if (n) *n = ql->n;
+    if (k) *k = ql->k;
+    if (group) *group = (size_t)ql->group;
+    if (has_bias) *has_bias = ql->bias != nullptr;
+    return NNE_OK;
+}
+
+size_t nne_qlinear4_memory_bytes(const nne_qlinear4 *ql) {
+    if (!ql) return 0;
+    return ql->tiles * ql->chunks * 32 * sizeof(uint4) + ql->tiles * padded_groups(ql->chunks, ql->group) * 8 * sizeof(float2) +
+           (ql->bias ? ql->n * sizeof(float) : 0);
+}
+
+int nne_qlinear4_forward_dev(nne_qlinear4 *ql, const float *x_dev, size_t m, size_t k, float *y_dev, void *stream) {
+    NNE_GUARD_BEGIN
+    return forward4(ql, x_dev, m, k, y_dev, ql ? ql->n : 0, (cudaStream_t)stream);
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_forward_dev_strided(nne_qlinear4 *ql, const float *x_dev, size_t m, size_t k, float *y_dev, size_t ldy, void *stream) {
+    NNE_GUARD_BEGIN
+    return forward4(ql, x_dev, m, k, y_dev, ldy, (cudaStream_t)stream);
+    NNE_GUARD_END
+}
+
+int nne_qlinear4_forward_host(nne_qlinear4 *ql, const float *x_host, size_t m, size_t k, float *y_host) {
+    NNE_GUARD_BEGIN
+    if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
+    if (k != ql->k) return fail(NNE_ERR_SHAPE_MISMATCH, "shape mismatch: expected [%zu], got [%zu]", ql->k, k);
+    size_t xb, yb;
+    if (__builtin_mul_overflow(m, ql->k, &xb) || __builtin_mul_overflow(xb, sizeof(float), &xb) ||
+        __builtin_mul_overflow(m, ql->n, &yb) || __builtin_mul_overflow(yb, sizeof(float), &yb))
+        return fail(NNE_ERR_INVALID_ARGUMENT, "m*k or m*n overflows size_t");
+    if (m == 0 || ql->n == 0) return NNE_OK;
+    if ((xb && !x_host) || !y_host) return fail(NNE_ERR_INVALID_ARGUMENT, "null host pointer");
+    nne_ctx *ctx = ql->ctx;
+    NNE_TRY(use_ctx(ctx));
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    NNE_TRY(ctx->stage_a.reserve(xb ? xb : 4));
+    NNE_TRY(ctx->stage_b.reserve(yb));
+    if (xb) NNE_CUDA_TRY(cudaMemcpyAsync(ctx->stage_a.ptr, x_host, xb, cudaMemcpyHostToDevice, ctx->stream));
+    NNE_TRY(forward4(ql, (const float *)ctx->stage_a.ptr, m, k, (float *)ctx->stage_b.ptr, ql->n, ctx->stream));
+    NNE_CUDA_TRY(cudaMemcpyAsync(y_host, ctx->stage_b.ptr, yb, cudaMemcpyDeviceToHost, ctx->stream));
+    NNE_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+    return NNE_OK;
+    NNE_GUARD_END
+}
+
+}  // extern "C"

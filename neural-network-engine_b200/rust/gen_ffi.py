@@ -15,8 +15,8 @@ HEADER = os.path.join(HERE, "..", "..", "include", "nne_cuda.h")
 OUT = os.path.join(HERE, "src", "gpu", "cuda", "ffi.rs")
 
 SCALARS = {"int": "c_int", "unsigned int": "c_uint", "size_t": "usize", "float": "f32", "int8_t": "i8",
-           "uint64_t": "u64", "void": "c_void", "char": "c_char"}
-OPAQUE = ["nne_ctx", "nne_qlinear", "nne_plan", "nne_shard_group"]
+           "uint8_t": "u8", "int32_t": "i32", "double": "f64", "uint64_t": "u64", "void": "c_void", "char": "c_char"}
+OPAQUE = ["nne_ctx", "nne_qlinear", "nne_qlinear4", "nne_plan", "nne_shard_group"]
 
 
 def rust_type(c: str) -> str:

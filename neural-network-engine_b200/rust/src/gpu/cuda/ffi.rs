@@ -12,6 +12,10 @@ pub struct nne_qlinear {
     _private: [u8; 0],
 }
 #[repr(C)]
+pub struct nne_qlinear4 {
+    _private: [u8; 0],
+}
+#[repr(C)]
 pub struct nne_plan {
     _private: [u8; 0],
 }
@@ -246,6 +250,91 @@ extern "C" {
         items: *const nne_plan_item,
         m: usize,
         out: *mut *mut nne_plan,
+    ) -> c_int;
+    pub fn nne_quantize_rows4_dev(
+        ctx: *mut nne_ctx,
+        w_dev: *const f32,
+        rows: usize,
+        cols: usize,
+        group: usize,
+        q_dev: *mut u8,
+        scales_dev: *mut f32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn nne_qlinear4_create_from_f32(
+        ctx: *mut nne_ctx,
+        w_host: *const f32,
+        bias_host_or_null: *const f32,
+        n: usize,
+        k: usize,
+        group: usize,
+        out: *mut *mut nne_qlinear4,
+    ) -> c_int;
+    pub fn nne_qlinear4_create_from_f32_dev(
+        ctx: *mut nne_ctx,
+        w_dev: *const f32,
+        bias_dev_or_null: *const f32,
+        n: usize,
+        k: usize,
+        group: usize,
+        stream: *mut c_void,
+        out: *mut *mut nne_qlinear4,
+    ) -> c_int;
+    pub fn nne_qlinear4_create_from_i4(
+        ctx: *mut nne_ctx,
+        q_host: *const u8,
+        scales_host: *const f32,
+        bias_host_or_null: *const f32,
+        n: usize,
+        k: usize,
+        group: usize,
+        out: *mut *mut nne_qlinear4,
+    ) -> c_int;
+    pub fn nne_qlinear4_create_from_i4_dev(
+        ctx: *mut nne_ctx,
+        q_dev: *const u8,
+        scales_dev: *const f32,
+        bias_dev_or_null: *const f32,
+        n: usize,
+        k: usize,
+        group: usize,
+        stream: *mut c_void,
+        out: *mut *mut nne_qlinear4,
+    ) -> c_int;
+    pub fn nne_qlinear4_destroy(ql: *mut nne_qlinear4) -> c_int;
+    pub fn nne_qlinear4_download(ql: *const nne_qlinear4, q_host: *mut u8, scales_host: *mut f32) -> c_int;
+    pub fn nne_qlinear4_dequantize(ql: *const nne_qlinear4, w_host: *mut f32) -> c_int;
+    pub fn nne_qlinear4_info(
+        ql: *const nne_qlinear4,
+        n: *mut usize,
+        k: *mut usize,
+        group: *mut usize,
+        has_bias: *mut c_int,
+    ) -> c_int;
+    pub fn nne_qlinear4_memory_bytes(ql: *const nne_qlinear4) -> usize;
+    pub fn nne_qlinear4_forward_host(
+        ql: *mut nne_qlinear4,
+        x_host: *const f32,
+        m: usize,
+        k: usize,
+        y_host: *mut f32,
+    ) -> c_int;
+    pub fn nne_qlinear4_forward_dev(
+        ql: *mut nne_qlinear4,
+        x_dev: *const f32,
+        m: usize,
+        k: usize,
+        y_dev: *mut f32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn nne_qlinear4_forward_dev_strided(
+        ql: *mut nne_qlinear4,
+        x_dev: *const f32,
+        m: usize,
+        k: usize,
+        y_dev: *mut f32,
+        ldy: usize,
+        stream: *mut c_void,
     ) -> c_int;
     pub fn nne_shard_group_create(
         ctx: *mut nne_ctx,
