@@ -307,11 +307,11 @@ NNE_API int nne_qlinear_plan_create_fused(nne_ctx *ctx, size_t count, const nne_
  * [n, ceil(k / group)].  No counterpart in the reference.
  *
  * A forward computes y[r,j] = sum_g scale[j,g] * sum_{i in g} q[j,i] * x[r,i] (+ bias[j]) with the
- * accuracy of f32: an activation enters as the sum of two 11-bit numbers (2^-22 of its group's largest
- * |x|), products are exact, sums are f32.  A row's result does not depend on which other rows are in
+ * accuracy of f32: an activation is put on a grid of its group (off by 2^-23 of the group's largest |x| at
+ * most), products and sums within a group are exact integers, sums over groups are f32.  A row's result does not depend on which other rows are in
  * the batch as long as the batch stays in one of the ranges 1..4, 5..8, 9..16, 17..32.  A row of x that
  * holds Inf or NaN gives NaN or Inf in every channel whose codes meet it; other rows are untouched.
- * One launch, no workspace.  Weights are read once for up to 32 rows, once more for each further 32.
+ * Up to four rows are one launch; more are two, with a stream-ordered workspace of about 4 * m * k bytes.  Weights are read once for up to 32 rows, once more for each further 32.
  * The handle is immutable and forwards may run concurrently, as with nne_qlinear.  Limits: 2^22 rows,
  * 2^30 columns. */
 NNE_API int nne_quantize_rows4_dev(nne_ctx *ctx, const float *w_dev, size_t rows, size_t cols, size_t group,

@@ -9,7 +9,7 @@
 // Public layout: codes [n, ceil(k/2)] bytes, two's complement, the even column in the low four bits; scales
 // [n, ceil(k/group)].  On the device the layer keeps one private copy, laid out for the forward kernel: tiles of
 // 16 rows x 64 columns, 512 bytes each, in which lane l's 16 bytes hold its operand fragments of four
-// m16n8k16 MMAs (a code as q + 8, so that three integer operations turn four codes into two f16 pairs), and the
+// m16n8k16 MMAs (a code as q + 8, which two integer operations make f16 pairs of), and the
 // scales as [tile][group][8][2] (rows r and r + 8 side by side: what one lane needs).  k is padded to 64 and n to
 // 16 with zero codes.
 #include <cuda_fp16.h>
@@ -35,7 +35,8 @@ namespace {
 
 constexpr int Q4_ROWS = 16;        // rows of a tile
 constexpr int Q4_CHUNK = 64;       // columns of a tile
-constexpr int Q4_WARPS = 8;        // row tiles (one a warp) of a CTA
+constexpr int Q4_DEPTH = 8;        // 512-byte weight loads a warp has on their way
+constexpr int Q4_PREP = 4;         // activation pieces whose loads a warp has on their way
 constexpr int Q4_MAX_SPLIT = 8;    // CTAs of a cluster that share a row block's columns
 
 __host__ __device__ inline size_t padded_groups(size_t chunks, int group) {
@@ -182,37 +183,32 @@ dequantize4_kernel(const uint4 *__restrict__ words, const float2 *__restrict__ s
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------
-// The weights are the 16-row side of mma.sync m16n8k16 (f16, exact: a code is an integer), the activations the
-// 8-column side.  An activation is the sum of two f16 numbers (columns 2r and 2r + 1 of a step: its rounding to
-// f16, and what that leaves), 22 bits, after a power of two that brings the largest |x| of its group of columns
-// to [2^13, 2^14): the product keeps f32's accuracy, where one f16 would give 2^-11.  Products are exact, sums are f32;
-// at a group's end the two columns are added and go into the row's sum with scale * 2^-e.
+// The weights are the 16-row side of mma.sync m16n8k16 (f16), the activations the 8-column side, and all a group
+// adds up is exact integers:
+//  - A code enters as q + 8 in 0..15, its four bits being the low mantissa bits of an f16 number: (q + 8) * 2^-24 (rows
+//    0..7 of a tile) or (q + 8) * 2^-20 (rows 8..15), exact subnormals that cost one AND for two codes.  The 8 comes
+//    off again through the MMA's initial accumulator, -8 * sum of the group's activations.
+//  - An activation is put on the grid 2^-e of its group, v = rint(x * 2^e), max|v| in [2^22, 2^23], and split as
+//    v = 4096 h + l, |h|, |l| <= 2048: two f16 integers, the columns 2r and 2r + 1.  (q + 8) h summed over 128 columns
+//    stays below 2^22, so the f32 accumulators hold the integer exactly.
+//  At a group's end 4096 * (hi sum) + (lo sum) rounds once and joins the row's f32 sum with scale * 2^-e.  The error is
+//  that of f32 (x off by 2^-23 of its group's largest); one f16 for x would give 2^-11.
 //
-// A CTA takes 128 rows (a tile a warp) and a share of the columns; the CTAs of a cluster take the shares of one
+// A CTA takes 128 or 256 rows (a tile a warp) and a share of the columns; the CTAs of a cluster take the shares of one
 // row block and add their sums up through each other's shared memory in rank order, so results do not change from
-// run to run, and no workspace is needed.  Each warp streams its weights straight into registers, Q4_DEPTH loads of
-// 512 bytes ahead, and they start before the wait for the kernel that makes x (a layer never changes).
+// run to run.  Each warp streams its weights through a ring of its own, filled by asynchronous copies seven tiles ahead
+// that start before the wait for the kernel that makes x (a layer never changes); no other warp is waited for.  (The same
+// ring in registers spilled, and a spilled load is a load waited for: 95 us instead of 47 on 8192 -> 28672, group 32.)  Up to four activation rows are put on the
+// grid by the CTAs themselves; more are put there once by a kernel before (q4_prepare_kernel): with 12 rows of
+// 4091 -> 11003 every CTA preparing its own share took 50 us in all.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Eight codes of a word as the four A registers of a step.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&a)[4]) {
-    const uint32_t h = w >> 8;
-    const uint32_t magic = 0x64006400u;  // 1024 + code, or 1024 + 16 * code
-    const __half2 off = __half2half2(__ushort_as_half(0xe408));    // -1032 = -(1024 + 8)
-    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
-    const __half2 off16 = __half2half2(__ushort_as_half(0xd480));  // -72 = -(1024 / 16 + 8)
-    uint32_t u[4] = {(w & 0x000f000fu) | magic, (w & 0x00f000f0u) | magic, (h & 0x000f000fu) | magic, (h & 0x00f000f0u) | magic};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __half2 v = *reinterpret_cast<__half2 *>(&u[i]);
-        v = (i & 1) ? __hfma2(v, sixteenth, off16) : __hadd2(v, off);
-        a[i] = *reinterpret_cast<uint32_t *>(&v);
-    }
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 struct Q4Args {
@@ -220,163 +216,275 @@ struct Q4Args {
     const float2 *scales;
     const float *bias, *x;
     float *y;
+    const uint8_t *frag;   // prepared activations [row block][chunk][CHUNK_BYTES], or null: the CTAs prepare theirs
+    const float4 *info;    // [row block][group][COLS]
     size_t n, k, m, ldy;
     unsigned tiles, chunks, pgroups;
     unsigned span;    // chunks of a CTA's share
-    unsigned stage;   // chunks whose activations are in shared memory at once
+    unsigned stage;   // chunks whose activations are in one shared-memory buffer
     int vec;          // rows of x can be read as float4
 };
 
 template <int NT>
 struct Q4Shape {
     static constexpr int COLS = 4 * NT;                  // activation rows of a CTA
-    static constexpr int DEPTH = NT >= 8 ? 4 : 8;        // weight loads in flight a lane
     static constexpr int CHUNK_BYTES = 4 * NT * 256;     // fragments of 64 columns
+    // Row tiles (one a warp) of a CTA.  With 32 activation rows a CTA has an SM to itself, so that a buffer of
+    // fragments serves twice the weight rows.
+    static constexpr int WARPS = NT >= 8 ? 16 : 8;
+    template <int GROUP>
+    __host__ __device__ static constexpr int slot() {  // bytes of a ring slot: codes, scales
+        return Q4_CHUNK * Q4_ROWS / 2 + (GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP) * 64;
+    }
 };
 
+// A piece is 128 columns of one activation row, four a lane: columns blk * 128 + lane * 4 ...
+__device__ __forceinline__ void q4_load_piece(const float *row, size_t c, size_t k, int vec, float (&v)[4]) {
+    v[0] = v[1] = v[2] = v[3] = 0.0f;
+    if (vec) {
+        if (c < k) {
+            const float4 f = *reinterpret_cast<const float4 *>(row + c);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < k) v[i] = row[c + i];
+    }
+}
+// The piece on its groups' grids.  `frag`: where the fragments of the lane's chunk start; r: row within the block.
+// Fragment words: [step pair][n-tile][lane][step of the pair][2].  `info` (lanes that start a group): the initial
+// accumulators -8 * sum of h and of l, and 2^-e for rows 0..7 and 8..15 of a tile, all in units of the MMA's products.
 template <int GROUP, int NT>
-__global__ void __launch_bounds__(Q4_WARPS * 32, 2) q4_forward_kernel(const Q4Args p) {
+__device__ __forceinline__ void q4_put_piece(const float (&v)[4], int lane, unsigned r, bool there, uint32_t *frag, float4 *info) {
+    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int o = 1; o < GROUP / 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // 2^e by its bits: top * 2^e in [2^22, 2^23); e stays within -105 .. 126, so that 2^e and 2^(20-e) are normal
+    int e = 22 + 127 - ((int)(__float_as_uint(top) >> 23) & 255);
+    e = e > 126 ? 126 : (e < -105 ? -105 : e);
+    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+    float h[4], l[4], hs = 0.0f, ls = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = rintf(v[i] * up);
+        h[i] = rintf(t * (1.0f / 4096.0f));
+        l[i] = fmaf(h[i], -4096.0f, t);
+        hs += h[i], ls += l[i];
+    }
+#pragma unroll
+    for (int o = 1; o < GROUP / 4; o <<= 1) {
+        hs += __shfl_xor_sync(0xffffffffu, hs, o);
+        ls += __shfl_xor_sync(0xffffffffu, ls, o);
+    }
+    if (!there) return;
+    const int kk = (lane & 3) * 4, step = (lane & 15) >> 2;
+    const int t = (kk & 7) / 2, word = kk >> 3, g = 2 * (r & 3);
+    uint32_t *f = frag + (((step >> 1) * NT + r / 4) * 32 + g * 4 + t) * 4 + (step & 1) * 2 + word;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // 16 h and 16 l: at most 32768, exact in f16
+        const __half2 hh = __floats2half2_rn(h[2 * i] * 16.0f, h[2 * i + 1] * 16.0f);
+        const __half2 ll = __floats2half2_rn(l[2 * i] * 16.0f, l[2 * i + 1] * 16.0f);
+        f[i * 4] = *reinterpret_cast<const uint32_t *>(&hh);
+        f[i * 4 + 16] = *reinterpret_cast<const uint32_t *>(&ll);
+    }
+    if ((lane * 4) % GROUP == 0)
+        *info = make_float4(hs * -0x1p-17f, ls * -0x1p-17f, __uint_as_float((uint32_t)(127 + 20 - e) << 23),
+                            __uint_as_float((uint32_t)(127 + 16 - e) << 23));
+}
+
+// Groups of 64-column chunk c's column `col`, counted from chunk c0 (a multiple of two).
+template <int GROUP>
+__device__ __forceinline__ unsigned q4_group(unsigned c, int col) {
+    return GROUP >= Q4_CHUNK ? c / (GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1) : c * (Q4_CHUNK / GROUP) + col / GROUP;
+}
+
+// Groups that start in the first c chunks.
+template <int GROUP>
+__host__ __device__ __forceinline__ unsigned q4_groups(unsigned c) {
+    return GROUP >= Q4_CHUNK ? (c + (GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1) - 1) / (GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1)
+                             : c * (Q4_CHUNK / GROUP);
+}
+
+template <int GROUP, int NT>
+__global__ void __launch_bounds__(256) q4_prepare_kernel(const Q4Args p, uint8_t *frag, float4 *info) {
+    constexpr int COLS = Q4Shape<NT>::COLS;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const unsigned blocks = (p.chunks + 1) / 2;
+    const size_t total = (size_t)blocks * p.m;
+    for (size_t b = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); b < total; b += (size_t)gridDim.x * 8) {
+        const size_t row = b / blocks;
+        const unsigned ck = 2 * (unsigned)(b - row * blocks) + (lane >> 4), r = (unsigned)(row % COLS);
+        const size_t mb = row / COLS;
+        float v[4];
+        q4_load_piece(p.x + row * p.k, (size_t)ck * Q4_CHUNK + (lane & 15) * 4, p.k, p.vec, v);
+        const bool there = ck < p.chunks;
+        q4_put_piece<GROUP, NT>(v, lane, r, there,
+                                reinterpret_cast<uint32_t *>(frag + (mb * p.chunks + ck) * Q4Shape<NT>::CHUNK_BYTES),
+                                info + (mb * p.pgroups + q4_group<GROUP>(ck, (lane & 15) * 4)) * COLS + r);
+    }
+}
+
+template <int GROUP, int NT, bool READY>
+__global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WARPS) q4_forward_kernel(const Q4Args p) {
     using S = Q4Shape<NT>;
-    constexpr int GPC = GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP;   // scale pairs a chunk needs
+    constexpr int WARPS = S::WARPS, ROWS = WARPS * Q4_ROWS, D = Q4_DEPTH;
+    constexpr int GPC = GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP;   // groups of a chunk
     constexpr int CPG = GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1;   // chunks of a group
-    constexpr int STEPS = GROUP >= Q4_CHUNK ? 4 : GROUP / 16;       // MMA steps between two group ends
+    constexpr int SLOT = S::template slot<GROUP>();
     extern __shared__ __align__(16) uint8_t smem[];
-    uint2 *frag = reinterpret_cast<uint2 *>(smem);                                       // [chunk][4][NT][32]
-    float *factor = reinterpret_cast<float *>(smem + (size_t)p.stage * S::CHUNK_BYTES);  // [group][COLS]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned split = gridDim.x, rank = blockIdx.x;
-    const unsigned tile = blockIdx.y * Q4_WARPS + warp;
+    const unsigned tile = blockIdx.y * WARPS + warp;
     const size_t row0 = (size_t)blockIdx.z * S::COLS;  // first activation row
-    const int cols = (int)(p.m - row0 < (size_t)S::COLS ? p.m - row0 : S::COLS);
+    const unsigned cols = (unsigned)(p.m - row0 < (size_t)S::COLS ? p.m - row0 : S::COLS);
     const unsigned c_begin = rank * p.span < p.chunks ? rank * p.span : p.chunks;
     const unsigned c_end = c_begin + p.span < p.chunks ? c_begin + p.span : p.chunks;
     const bool mine = tile < p.tiles;
 
-    const uint4 *wp = p.words + ((size_t)(mine ? tile : 0) * p.chunks) * 32 + lane;
-    const float2 *sp = p.scales + (size_t)(mine ? tile : 0) * p.pgroups * 8 + (lane >> 2);
-    uint4 ring[S::DEPTH];
-    float2 sring[S::DEPTH][GPC];
-    auto fetch = [&](unsigned c, uint4 &w, float2 (&s)[GPC]) {
-        if (mine && c < c_end) {
-            w = __ldcs(wp + (size_t)c * 32);
-#pragma unroll
-            for (int g = 0; g < GPC; ++g) s[g] = __ldg(sp + ((size_t)(c / CPG) * GPC + g) * 8);
-        } else {
-            w = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int g = 0; g < GPC; ++g) s[g] = make_float2(0.0f, 0.0f);
+    // The warp's ring of weight tiles: slot j holds chunk c with (c - c_begin) % D == j, a lane's 16 bytes copied by
+    // that lane, and behind the codes the scales of the chunk's groups.  One copy group a chunk, also where a chunk has
+    // no copy to make, so that "all but the last D - 2 groups" is always chunk c.
+    uint8_t *ring = smem + warp * (D * SLOT);
+    uint8_t *xbuf = smem + WARPS * D * SLOT;
+    const uint32_t ring_at = smem_u32(ring) + lane * 16;
+    const uint4 *wp = p.words + ((size_t)(mine ? tile : 0) * p.chunks + c_begin) * 32 + lane;
+    const float2 *sp = p.scales + ((size_t)(mine ? tile : 0) * p.pgroups + q4_group<GROUP>(c_begin, 0)) * 8 + lane * 2;
+    // chunk c_begin + at + j: `at` a multiple of D, so that the slot and the offsets are known when compiled
+    auto fetch = [&](unsigned at, int j, bool there) {
+        if (there) {
+            cp_async_16(ring_at + (j % D) * SLOT, wp + (size_t)at * 32 + j * 32);
+            if (lane < GPC * 4) cp_async_16(ring_at + (j % D) * SLOT + 512, sp + (size_t)(at / CPG * GPC) * 8 + (j / CPG) * GPC * 8);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    const unsigned share = c_end - c_begin;
 #pragma unroll
-    for (int j = 0; j < S::DEPTH; ++j) fetch(c_begin + j, ring[j], sring[j]);
+    for (int j = 0; j < D - 1; ++j) fetch(0, j, mine && (unsigned)j < share);
 
     grid_dependency_wait();
     grid_launch_dependents();
 
     float sum[NT][2], part[NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        sum[t][0] = sum[t][1] = 0.0f;
-        part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.0f;
+    for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = 0.0f;
+
+    // Prepared activations of the chunks from s0 (counted in the share) on: 16-byte copies into buffer `buf`, part of
+    // the copy group that is committed next.
+    const unsigned buf_bytes = p.stage * S::CHUNK_BYTES + q4_groups<GROUP>(p.stage) * S::COLS * (unsigned)sizeof(float4);
+    auto copy_in = [&](unsigned s0, unsigned buf) {
+        const unsigned s1 = s0 + p.stage < share ? s0 + p.stage : share;
+        const uint32_t dst = smem_u32(xbuf) + buf * buf_bytes;
+        const uint8_t *src = p.frag + (blockIdx.z * (size_t)p.chunks + c_begin + s0) * S::CHUNK_BYTES;
+        for (unsigned i = threadIdx.x; i < (s1 - s0) * (S::CHUNK_BYTES / 16); i += WARPS * 32) cp_async_16(dst + i * 16, src + (size_t)i * 16);
+        const float4 *isrc = p.info + (blockIdx.z * (size_t)p.pgroups + q4_group<GROUP>(c_begin + s0, 0)) * S::COLS;
+        for (unsigned i = threadIdx.x; i < q4_groups<GROUP>(s1 - s0) * S::COLS; i += WARPS * 32)
+            cp_async_16(dst + p.stage * S::CHUNK_BYTES + i * 16, isrc + i);
+    };
+
+    unsigned buf = 0;
+    for (unsigned s0 = 0; s0 < share; s0 += p.stage) {
+        const unsigned s1 = s0 + p.stage < share ? s0 + p.stage : share;
+        uint8_t *here = xbuf + buf * buf_bytes;
+        float4 *info = reinterpret_cast<float4 *>(here + p.stage * S::CHUNK_BYTES);  // [group][COLS]
+        if (READY) {
+            if (s0 == 0) {
+                copy_in(0, 0);
+                asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+            } else if (!mine) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncthreads();  // this stage's copies (D chunks old) are there for everybody, the other buffer is free
+            if (s1 < share) copy_in(s1, buf ^ 1);
+            buf ^= 1;
+        } else {
+            // Columns of rows that are not there keep whatever the memory held: the sums they lead to are not stored.
+            if (s0 != 0) __syncthreads();
+            const unsigned pieces = ((s1 - s0 + 1) / 2) * cols;
+            for (unsigned b0 = warp; b0 < pieces; b0 += WARPS * Q4_PREP) {
+                float v[Q4_PREP][4];
+#pragma unroll
+                for (int u = 0; u < Q4_PREP; ++u) {
+                    const unsigned b = b0 + u * WARPS, ck = c_begin + s0 + 2 * (b / cols) + (lane >> 4);
+                    v[u][0] = v[u][1] = v[u][2] = v[u][3] = 0.0f;
+                    if (b < pieces && ck < c_begin + s1)
+                        q4_load_piece(p.x + (row0 + b % cols) * p.k, (size_t)ck * Q4_CHUNK + (lane & 15) * 4, p.k, p.vec, v[u]);
+                }
+#pragma unroll
+                for (int u = 0; u < Q4_PREP; ++u) {
+                    const unsigned b = b0 + u * WARPS, r = b % cols;
+                    if (b >= pieces) break;  // the same for the whole warp
+                    const unsigned ck = 2 * (b / cols) + (lane >> 4);
+                    q4_put_piece<GROUP, NT>(v[u], lane, r, s0 + ck < s1, reinterpret_cast<uint32_t *>(here + ck * S::CHUNK_BYTES),
+                                            info + q4_group<GROUP>(ck, (lane & 15) * 4) * S::COLS + r);
+                }
+            }
+            __syncthreads();
+        }
+        if (!mine) {  // a warp behind the last tile only helps to prepare
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            continue;
+        }
+
+        // Chunk at + j of the share; `end`: the last one of an unfinished group of 128 columns.
+        auto chunk = [&](unsigned at, int j, bool more, bool end) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+            __syncwarp();  // the slot's scales are there for every lane, and the slot before has been read by every lane
+            fetch(at, j + D - 1, more);
+            const uint8_t *slot = ring + j * SLOT;
+            const uint4 w4 = reinterpret_cast<const uint4 *>(slot)[lane];
+            const float2 *sc = reinterpret_cast<const float2 *>(slot + 512) + (lane >> 2);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const uint4 *fc = reinterpret_cast<const uint4 *>(here + (at - s0) * S::CHUNK_BYTES) + j * (S::CHUNK_BYTES / 16) + lane;
+            const float4 *ic = info + (at - s0) / CPG * GPC * S::COLS + (lane & 3);
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+                uint32_t a[2][4];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t lo = w[2 * pair + q], up = lo >> 8;
+                    a[q][0] = lo & 0x000f000fu, a[q][1] = lo & 0x00f000f0u, a[q][2] = up & 0x000f000fu, a[q][3] = up & 0x00f000f0u;
+                }
+                const bool first = pair == 0 ? (CPG == 1 || j % CPG == 0) : GPC == 2;
+                const bool last = pair == 0 ? GPC == 2 : (CPG == 1 || j % CPG == CPG - 1 || end);
+                const int grp = CPG > 1 ? j / CPG : j * GPC + (GPC == 2 ? pair : 0);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint4 b = fc[(pair * NT + t) * 32];
+                    if (first) {
+                        const float2 i0 = *reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4);
+                        part[t][0] = i0.x, part[t][1] = i0.y, part[t][2] = 16.0f * i0.x, part[t][3] = 16.0f * i0.y;
+                    }
+                    mma_f16(part[t], a[0], b.x, b.y);
+                    mma_f16(part[t], a[1], b.z, b.w);
+                }
+                if (last) {
+                    const float2 s2 = sc[GPC == 2 ? pair * 8 : 0];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const float2 f = *(reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4) + 1);
+                        sum[t][0] = fmaf(s2.x * f.x, fmaf(part[t][0], 4096.0f, part[t][1]), sum[t][0]);
+                        sum[t][1] = fmaf(s2.y * f.y, fmaf(part[t][2], 4096.0f, part[t][3]), sum[t][1]);
+                    }
+                }
+            }
+        };
+        unsigned at = s0;
+        for (; at + 2 * D <= share && at + D <= s1; at += D) {  // rounds whose fetches all exist
+#pragma unroll
+            for (int j = 0; j < D; ++j) chunk(at, j, true, false);
+        }
+        for (; at < s1; at += D) {
+#pragma unroll
+            for (int j = 0; j < D; ++j)
+                if (at + j < s1) chunk(at, j, at + j + D - 1 < share, at + j + 1 == share);
+        }
     }
 
-    for (unsigned s0 = c_begin; s0 < c_end; s0 += p.stage) {
-        const unsigned s1 = s0 + p.stage < c_end ? s0 + p.stage : c_end;
-        // Activations of these chunks: a warp takes 128 columns of one row at a time, four a lane.
-        if (s0 != c_begin) __syncthreads();
-        const unsigned blocks = (s1 - s0 + 1) / 2;
-        for (unsigned b = warp; b < blocks * S::COLS; b += Q4_WARPS) {
-            const unsigned r = b % S::COLS, blk = b / S::COLS;
-            const unsigned ck = s0 + 2 * blk + (lane >> 4);  // this lane's chunk
-            const size_t c = (size_t)ck * Q4_CHUNK + (lane & 15) * 4;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if ((int)r < cols && ck < s1) {
-                const float *src = p.x + (row0 + r) * p.k + c;
-                if (p.vec) {
-                    if (c < p.k) {
-                        const float4 f = *reinterpret_cast<const float4 *>(src);
-                        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c + i < p.k) v[i] = src[i];
-                }
-            }
-            float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-            for (int o = 1; o < GROUP / 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // 2^e by its bits: top * 2^e in [2^13, 2^14); e within -114 .. 126 keeps 2^e and 2^-e normal
-            const int be = (int)(__float_as_uint(top) >> 23) & 255;
-            int e = 13 + 127 - be;
-            e = e > 126 ? 126 : (e < -114 ? -114 : e);
-            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-            if (ck < s1) {
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float a = v[2 * h] * up, d = v[2 * h + 1] * up;
-                    const __half2 hh = __floats2half2_rn(a, d);
-                    const float2 back = __half22float2(hh);
-                    const __half2 ll = __floats2half2_rn(a - back.x, d - back.y);
-                    hi[h] = *reinterpret_cast<const uint32_t *>(&hh);
-                    lo[h] = *reinterpret_cast<const uint32_t *>(&ll);
-                }
-                const int kk = (lane & 3) * 4, step = (lane & 15) >> 2;
-                const int t = (kk & 7) / 2, word = kk >> 3, g = 2 * (r & 3);
-                uint32_t *f = reinterpret_cast<uint32_t *>(frag + (((size_t)(ck - s0) * 4 + step) * NT + r / 4) * 32);
-                f[(g * 4 + t) * 2 + word] = hi[0];
-                f[(g * 4 + t + 1) * 2 + word] = hi[1];
-                f[((g + 1) * 4 + t) * 2 + word] = lo[0];
-                f[((g + 1) * 4 + t + 1) * 2 + word] = lo[1];
-                if ((lane * 4) % GROUP == 0) {
-                    const unsigned grp = GROUP >= Q4_CHUNK ? (ck - s0) / CPG : (ck - s0) * GPC + ((lane & 15) * 4) / GROUP;
-                    factor[(size_t)grp * S::COLS + r] = __uint_as_float((uint32_t)(127 - e) << 23);
-                }
-            }
-        }
-        __syncthreads();
-
-        for (unsigned base = s0; base < s1; base += S::DEPTH) {
-#pragma unroll
-            for (int j = 0; j < S::DEPTH; ++j) {
-                const unsigned c = base + j;
-                if (c < s1) {  // the same for the whole CTA
-                    const uint4 w4 = ring[j];
-                    float2 sc[GPC];
-#pragma unroll
-                    for (int g = 0; g < GPC; ++g) sc[g] = sring[j][g];
-                    fetch(c + S::DEPTH, ring[j], sring[j]);
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-                    const uint2 *fc = frag + (size_t)(c - s0) * 4 * NT * 32 + lane;
-#pragma unroll
-                    for (int st = 0; st < 4; ++st) {
-                        uint32_t a[4];
-                        codes_to_f16(w[st], a);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const uint2 b = fc[(st * NT + t) * 32];
-                            mma_f16(part[t], a, b.x, b.y);
-                        }
-                        if (st % STEPS == STEPS - 1 && (CPG == 1 || ((c - s0) % CPG) == CPG - 1 || c + 1 == c_end)) {
-                            const float2 s2 = sc[GPC == 1 ? 0 : st / STEPS];
-                            const unsigned grp = CPG > 1 ? (c - s0) / CPG : (c - s0) * GPC + st / STEPS;
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                const float f = factor[(size_t)grp * S::COLS + t * 4 + (lane & 3)];
-                                sum[t][0] = fmaf(s2.x * f, part[t][0] + part[t][1], sum[t][0]);
-                                sum[t][1] = fmaf(s2.y * f, part[t][2] + part[t][3], sum[t][1]);
-                                part[t][0] = part[t][1] = part[t][2] = part[t][3] = 0.0f;
-                            }
-                        }
-                    }
-                }
-            }
-        }
-    }
-
-    // Sums of the cluster's CTAs: each leaves [128][COLS] in its shared memory, and rank i adds up every
-    // split-th row of all of them, rank after rank.
+    // Sums of the cluster's CTAs: each leaves [ROWS][COLS] in its shared memory, and rank i adds up its share of the
+    // rows of all of them, rank after rank.
     float *mysum = reinterpret_cast<float *>(smem);
     __syncthreads();
 #pragma unroll
@@ -389,12 +497,12 @@ __global__ void __launch_bounds__(Q4_WARPS * 32, 2) q4_forward_kernel(const Q4Ar
     } else {
         __syncthreads();
     }
-    const size_t out0 = (size_t)blockIdx.y * (Q4_WARPS * Q4_ROWS);
-    const unsigned per = (Q4_WARPS * Q4_ROWS + split - 1) / split;  // rows of this rank
-    for (unsigned i = threadIdx.x; i < per * S::COLS; i += Q4_WARPS * 32) {
+    const size_t out0 = (size_t)blockIdx.y * ROWS;
+    const unsigned per = (ROWS + split - 1) / split;  // rows of this rank
+    for (unsigned i = threadIdx.x; i < per * cols; i += WARPS * 32) {
         // neighbouring threads take neighbouring rows: y is written in runs along n
         const unsigned r = rank * per + i % per, c = i / per;
-        if (r >= Q4_WARPS * Q4_ROWS || out0 + r >= p.n || (int)c >= cols) continue;
+        if (r >= ROWS || out0 + r >= p.n) continue;
         float v = 0.0f;
         const uint32_t at = smem_u32(mysum + r * S::COLS + c);
         for (unsigned q = 0; q < split; ++q) {
@@ -414,23 +522,27 @@ __global__ void __launch_bounds__(Q4_WARPS * 32, 2) q4_forward_kernel(const Q4Ar
 template <int GROUP, int NT>
 int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
     using S = Q4Shape<NT>;
+    constexpr bool READY = NT > 1;
     const nne_ctx *ctx = ql->ctx;
-    const size_t blocks_n = (ql->tiles + Q4_WARPS - 1) / Q4_WARPS;
+    const size_t blocks_n = (ql->tiles + S::WARPS - 1) / S::WARPS;
     const size_t blocks_m = (m + S::COLS - 1) / S::COLS;
     if (blocks_n > 65535 || blocks_m > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "layer or batch too large for one launch");
-    // Split the columns until two CTAs an SM are there, as long as a share keeps four chunks of 64.
-    const size_t want = 2 * (size_t)ctx->sm_count, have = blocks_n * blocks_m;
-    unsigned split = (unsigned)((want + have - 1) / have);
-    if (split > Q4_MAX_SPLIT) split = Q4_MAX_SPLIT;
-    while (split > 1 && ql->chunks < (size_t)split * 4) --split;
+    // Split the columns over as many CTAs as the GPU holds at once - one more and a second round would run nearly
+    // empty (28672 -> 8192, one row, group 64, in 320 CTAs: 54 us, in 256: 31) - as long as a share keeps eight chunks of 64.
+    const size_t slots = (size_t)ctx->sm_count * (16 / S::WARPS), have = blocks_n * blocks_m;
+    size_t split = slots / have;
+    split = split < 1 ? 1 : (split > Q4_MAX_SPLIT ? Q4_MAX_SPLIT : split);
+    while (split > 1 && ql->chunks < split * 8) --split;
     // shares in whole pairs of chunks, so that a group of 128 columns never lies in two
     size_t span = (ql->chunks + split - 1) / split;
     span = (span + 1) & ~(size_t)1;
-    split = (unsigned)((ql->chunks + span - 1) / span);
-    // activations staged at once: at most 96 KB, so that two CTAs fit an SM
-    size_t stage = (size_t)98304 / (S::CHUNK_BYTES + 2 * S::COLS * sizeof(float));
-    stage = stage & ~(size_t)7;  // whole rounds of the register ring
-    if (stage > span) stage = span;
+    split = (ql->chunks + span - 1) / span;
+    // Activations in shared memory beside the weight rings, in stages of whole ring rounds: two buffers for prepared
+    // ones (the next stage is copied in during this one), one for those the CTA prepares.
+    const size_t ring = (size_t)S::WARPS * Q4_DEPTH * S::template slot<GROUP>();
+    auto xbytes = [](size_t chunks) { return chunks * S::CHUNK_BYTES + q4_groups<GROUP>((unsigned)chunks) * S::COLS * sizeof(float4); };
+    size_t stage = READY ? Q4_DEPTH : 7 * Q4_DEPTH;
+    if (stage >= span) stage = span;
     Q4Args a = {};
     a.words = ql->words;
     a.scales = ql->scales;
@@ -447,31 +559,46 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
     a.span = (unsigned)span;
     a.stage = (unsigned)stage;
     a.vec = ql->k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    size_t bytes = stage * S::CHUNK_BYTES + (stage * Q4_CHUNK / GROUP + 1) * S::COLS * sizeof(float);
-    const size_t sums = (size_t)Q4_WARPS * Q4_ROWS * S::COLS * sizeof(float);
+    size_t bytes = ring + xbytes(stage) * (READY && stage < span ? 2 : 1);
+    const size_t sums = (size_t)S::WARPS * Q4_ROWS * S::COLS * sizeof(float);
     if (bytes < sums) bytes = sums;
-    NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT>, bytes));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split, (unsigned)blocks_n, (unsigned)blocks_m);
-    cfg.blockDim = dim3(Q4_WARPS * 32);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = s;
+    NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT, READY>, bytes));
+
     cudaLaunchAttribute attr[2];
-    int na = 0;
-    attr[na].id = cudaLaunchAttributeClusterDimension;
-    attr[na].val.clusterDim.x = split;
-    attr[na].val.clusterDim.y = 1;
-    attr[na].val.clusterDim.z = 1;
-    ++na;
-    if (pdl_enabled()) {
-        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[na].val.programmaticStreamSerializationAllowed = 1;
-        ++na;
-    }
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
     cfg.attrs = attr;
-    cfg.numAttrs = na;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_forward_kernel<GROUP, NT>, a);
-    count_launch();
+    cfg.stream = s;
+    cudaError_t e = cudaSuccess;
+    void *work = nullptr;
+    if (READY) {
+        const size_t fb = blocks_m * ql->chunks * S::CHUNK_BYTES, ib = blocks_m * a.pgroups * S::COLS * sizeof(float4);
+        NNE_CUDA_TRY(cudaMallocAsync(&work, fb + ib, s));
+        uint8_t *frag = static_cast<uint8_t *>(work);
+        float4 *info = reinterpret_cast<float4 *>(frag + fb);
+        a.frag = frag;
+        a.info = info;
+        const size_t pieces = (ql->chunks + 1) / 2 * m, cap = (size_t)ctx->sm_count * 8;
+        cfg.gridDim = dim3((unsigned)((pieces + 7) / 8 < cap ? (pieces + 7) / 8 : cap));
+        cfg.blockDim = dim3(256);
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, q4_prepare_kernel<GROUP, NT>, a, frag, info);
+        count_launch();
+    }
+    if (e == cudaSuccess) {
+        cfg.gridDim = dim3((unsigned)split, (unsigned)blocks_n, (unsigned)blocks_m);
+        cfg.blockDim = dim3(S::WARPS * 32);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, q4_forward_kernel<GROUP, NT, READY>, a);
+        count_launch();
+    }
+    if (work) cudaFreeAsync(work, s);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(NNE_ERR_CUDA, "4-bit forward launch failed: %s", cudaGetErrorString(e));

@@ -1,11 +1,11 @@
 """The 4-bit layer (QLinear4) on the device against numpy in 64 bits: codes and scales bit for bit, forwards within
 a bound that counts the kernel's roundings.
 
-Forward bound, per element, in units of S = sum_i |x_i * q_i| * scale:  an activation is kept as two f16 numbers,
-off by at most 2^-22 |x| + 2^-38 max|x of its group|; the group's sum is built by group / 16 MMAs, whose f32 sums
-are each off by at most 2^-22 of the partial sum (the unit may truncate); scale * 2^-e and the two products are two
-roundings of 2^-24; the row's sum takes one f32 step a group, 2^-24 each, and at most 8 more between CTAs.  A group whose
-codes are all small beside its largest |x| has the second term as max|x_g| * sum|q| * scale."""
+Forward bound, per element.  An activation is rounded to its group's grid, whose step is at most 2^-22 of the group's
+largest |x|: off by 2^-23 of that, times sum|q| * scale.  Products and sums within a group are exact integers.  In units
+of S = sum_i |x_i * q_i| * scale, plus that rounding again: joining the two halves of a group's sum is one rounding of
+2^-24, scale * 2^-e exact, the row's sum one f32 step a group and at most 10 more between CTAs and for the bias.  A
+group whose offset part (8 times the sum of x) cancels costs nothing: it is exact."""
 import ctypes as C
 
 import numpy as np
@@ -55,7 +55,7 @@ def exact(codes, scales, group, x, bias):
     if bias is not None:
         y = y + bias
         s = s + np.abs(bias)
-    bound = s * (2.0 ** -22 + (group // 16) * 2.0 ** -22 + 4 * 2.0 ** -24 + (groups + 10) * 2.0 ** -24) + floor * 2.0 ** -38
+    bound = s * (groups + 12) * 2.0 ** -24 + floor * 2.0 ** -23 * 1.001
     return y, bound + 1e-37
 
 
