@@ -54,6 +54,7 @@ typedef enum nne_status {
 typedef struct nne_ctx nne_ctx;         /* one per device: streams, staging, SM count   */
 typedef struct nne_qlinear nne_qlinear; /* one device-resident int8 layer               */
 typedef struct nne_qlinear4 nne_qlinear4; /* one device-resident 4-bit layer            */
+typedef struct nne_kv_cache nne_kv_cache; /* a paged cache of keys and values           */
 typedef struct nne_plan nne_plan;       /* a fixed list of forwards run as one launch   */
 typedef struct nne_shard_group nne_shard_group; /* one rank's end of a column-shard exchange */
 
@@ -342,6 +343,70 @@ NNE_API int nne_qlinear4_forward_dev(nne_qlinear4 *ql, const float *x_dev, size_
                                      void *stream);
 NNE_API int nne_qlinear4_forward_dev_strided(nne_qlinear4 *ql, const float *x_dev, size_t m, size_t k,
                                              float *y_dev, size_t ldy, void *stream);
+
+/* ---- paged key/value cache ----------------------------------------------------------------------
+ * What a decoder block does between its q/k/v projections (src/models/llama.rs:226-228) and its output
+ * projection, with keys and values in pages.  A pool is [pages][kv_heads][page_size][head_dim] of 16-bit
+ * numbers; place i of a sequence lies in page page_table[sequence][i / page_size], at i % page_size.
+ * head_dim is 64, 96, 128 or 256, page_size a power of two from 8 to 1024, pages * kv_heads * page_size
+ * below 2^31.  rope_dims (a multiple of 8; 0: no rotation) is how many of a head's dimensions are rotated
+ * by position, as pairs (i, i + rope_dims/2) or, interleaved, (2i, 2i + 1), pair i by position *
+ * rope_base^(-2i / rope_dims), or by position * rope_freq[i] where rope_freq (host, rope_dims/2 numbers,
+ * copied) is given.  The pools are the caller's (16-byte aligned device pointers that outlive the handle)
+ * or, both NULL, the handle's own, zero-filled.  The handle is immutable; what the pools hold is ordered by
+ * the streams of the calls that write and read them. */
+enum { NNE_F16 = 1, NNE_BF16 = 2 };
+typedef struct nne_kv_cache_desc {
+    void *k_pages;
+    void *v_pages;
+    size_t pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+    int dtype;             /* NNE_F16 or NNE_BF16 */
+    int rope_dims;
+    int rope_interleaved;
+    double rope_base;
+    const double *rope_freq;
+} nne_kv_cache_desc;
+NNE_API int nne_kv_cache_create(nne_ctx *ctx, const nne_kv_cache_desc *desc, nne_kv_cache **out);
+NNE_API int nne_kv_cache_destroy(nne_kv_cache *cache);
+/* The pools and the bytes of each; any out pointer may be NULL. */
+NNE_API int nne_kv_cache_info(const nne_kv_cache *cache, void **k_pages, void **v_pages, size_t *bytes_each);
+
+/* One pass over the q, k and v of `tokens` tokens: RMSNorm of each query and key head over head_dim (where a
+ * gamma [head_dim] is given; the arithmetic of nne_rmsnorm_dev), rotation of queries and keys, queries to
+ * q_out in f32, keys and values to their pages, rounded once.  f32 inputs [tokens][heads][head_dim] with a
+ * stride in floats from token to token, so that the three may lie in one row of a fused projection.  q (with
+ * q_out, q_heads) or k and v may be left out.  q_out is [tokens][q_heads][head_dim] without gaps and may be q
+ * itself where q_stride is q_heads * head_dim; otherwise it overlaps no input.  sequence[t] is the row of
+ * page_table [sequences][table_stride], index[t] the place in the sequence, position[t] what the rotation goes by
+ * (NULL: index; drafted nodes of a tree share positions but not places).  A token with index[t] < 0 is padding:
+ * nothing of it is read beyond that or written.  Where the sequence, the place or the page that the table names does not
+ * exist, the token's key and value are not stored (its query is).  A place given twice in one call holds
+ * one of the two tokens' values, element by element, afterwards.  index may be NULL when only queries are
+ * given.  One launch, no workspace, asynchronous on `stream`. */
+typedef struct nne_kv_append {
+    const float *q;
+    const float *k;
+    const float *v;
+    float *q_out;
+    size_t q_stride;
+    size_t k_stride;
+    size_t v_stride;
+    size_t tokens;
+    int q_heads;
+    float eps;
+    const float *q_gamma;
+    const float *k_gamma;
+    const int32_t *page_table;
+    size_t table_stride;
+    int sequences;
+    const int32_t *sequence;
+    const int32_t *index;
+    const int32_t *position;
+} nne_kv_append;
+NNE_API int nne_kv_append_dev(nne_kv_cache *cache, const nne_kv_append *args, void *stream);
 
 /* ---- column shards over the GPUs of one node -------------------------------------------------
  * The reference has no multi-device code.  Its forward computes output channel j from row j of

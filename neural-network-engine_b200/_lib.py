@@ -99,6 +99,10 @@ SIGNATURES = {
     "nne_qlinear4_forward_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),
     "nne_qlinear4_forward_dev_strided": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p,
                                                    C.c_size_t, C.c_void_p]),
+    "nne_kv_cache_create": (C.c_int, [C.c_void_p, C.c_void_p, c_void_pp]),
+    "nne_kv_cache_destroy": (C.c_int, [C.c_void_p]),
+    "nne_kv_cache_info": (C.c_int, [C.c_void_p, c_void_pp, c_void_pp, C.POINTER(C.c_size_t)]),
+    "nne_kv_append_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "nne_shard_group_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, c_void_pp]),
     "nne_shard_group_handle": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nne_shard_group_connect": (C.c_int, [C.c_void_p, C.c_void_p]),
@@ -123,7 +127,24 @@ class PlanItem(C.Structure):
                 ("eps", C.c_float), ("gamma", C.c_void_p), ("x2", C.c_void_p), ("residual", C.c_void_p)]
 
 
+class KvCacheDesc(C.Structure):
+    """nne_kv_cache_desc of include/nne_cuda.h."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("pages", C.c_size_t), ("page_size", C.c_int),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_int), ("rope_dims", C.c_int),
+                ("rope_interleaved", C.c_int), ("rope_base", C.c_double), ("rope_freq", C.c_void_p)]
+
+
+class KvAppendArgs(C.Structure):
+    """nne_kv_append of include/nne_cuda.h."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_size_t),
+                ("k_stride", C.c_size_t), ("v_stride", C.c_size_t), ("tokens", C.c_size_t), ("q_heads", C.c_int),
+                ("eps", C.c_float), ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p), ("page_table", C.c_void_p),
+                ("table_stride", C.c_size_t), ("sequences", C.c_int), ("sequence", C.c_void_p), ("index", C.c_void_p),
+                ("position", C.c_void_p)]
+
+
 INPUT_PLAIN, INPUT_RMSNORM, INPUT_SILU_MUL = 0, 1, 2
+F16, BF16 = 1, 2
 
 _lib = None
 

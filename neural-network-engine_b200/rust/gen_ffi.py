@@ -16,7 +16,7 @@ OUT = os.path.join(HERE, "src", "gpu", "cuda", "ffi.rs")
 
 SCALARS = {"int": "c_int", "unsigned int": "c_uint", "size_t": "usize", "float": "f32", "int8_t": "i8",
            "uint8_t": "u8", "int32_t": "i32", "double": "f64", "uint64_t": "u64", "void": "c_void", "char": "c_char"}
-OPAQUE = ["nne_ctx", "nne_qlinear", "nne_qlinear4", "nne_plan", "nne_shard_group"]
+OPAQUE = ["nne_ctx", "nne_qlinear", "nne_qlinear4", "nne_kv_cache", "nne_plan", "nne_shard_group"]
 
 
 def rust_type(c: str) -> str:
@@ -59,14 +59,23 @@ def parse(header_text: str):
                 pm = re.match(r"(.*?)(\w+)$", p)
                 args.append((pm.group(2), rust_type(pm.group(1).strip())))
         funcs.append((name, rust_type(ret), args))
+    structs = []
+    for m in re.finditer(r"typedef struct (nne_\w+) \{(.*?)\} \1;", text, flags=re.S):
+        fields = []
+        for f in m.group(2).split(";"):
+            fm = re.match(r"(.*?)(\w+)$", " ".join(f.split()))
+            if fm:
+                fields.append((fm.group(2), rust_type(fm.group(1).strip())))
+        if m.group(1) != "nne_plan_item":  # written out below, with its own comment
+            structs.append((m.group(1), fields))
     statuses = re.findall(r"(NNE_(?:OK|ERR_\w+))\s*=\s*(\d+)", text)
-    inputs = re.findall(r"(NNE_INPUT_\w+)\s*=\s*(\d+)", text)
+    inputs = re.findall(r"(NNE_INPUT_\w+|NNE_B?F16)\s*=\s*(\d+)", text)
     handle_bytes = re.search(r"#define\s+NNE_SHARD_HANDLE_BYTES\s+(\d+)", text).group(1)
-    return funcs, statuses, inputs, handle_bytes
+    return funcs, statuses, inputs, handle_bytes, structs
 
 
 def generate(header_text: str) -> str:
-    funcs, statuses, inputs, handle_bytes = parse(header_text)
+    funcs, statuses, inputs, handle_bytes, structs = parse(header_text)
     out = ["//! Raw bindings of `include/nne_cuda.h`: one declaration per exported symbol, nothing else.",
            "//! GENERATED by `gen_ffi.py` from the header - edit the header, then run the generator.",
            "#![allow(non_camel_case_types)]",
@@ -77,6 +86,9 @@ def generate(header_text: str) -> str:
             "pub struct nne_plan_item {", "    pub layer: *mut nne_qlinear,", "    pub x: *const f32,",
             "    pub y: *mut f32,", "    pub input_op: c_int,", "    pub eps: f32,", "    pub gamma: *const f32,",
             "    pub x2: *const f32,", "    pub residual: *const f32,", "}", ""]
+    for name, fields in structs:
+        out += [f"/// `{name}`.", "#[repr(C)]", "#[derive(Clone, Copy)]", f"pub struct {name} {{"]
+        out += [f"    pub {f}: {t}," for f, t in fields] + ["}", ""]
     for name, val in statuses + inputs:
         out.append(f"pub const {name}: c_int = {val};")
     out += [f"pub const NNE_SHARD_HANDLE_BYTES: usize = {handle_bytes};", "", 'extern "C" {']

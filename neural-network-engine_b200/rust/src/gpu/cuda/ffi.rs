@@ -16,6 +16,10 @@ pub struct nne_qlinear4 {
     _private: [u8; 0],
 }
 #[repr(C)]
+pub struct nne_kv_cache {
+    _private: [u8; 0],
+}
+#[repr(C)]
 pub struct nne_plan {
     _private: [u8; 0],
 }
@@ -38,6 +42,47 @@ pub struct nne_plan_item {
     pub residual: *const f32,
 }
 
+/// `nne_kv_cache_desc`.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct nne_kv_cache_desc {
+    pub k_pages: *mut c_void,
+    pub v_pages: *mut c_void,
+    pub pages: usize,
+    pub page_size: c_int,
+    pub kv_heads: c_int,
+    pub head_dim: c_int,
+    pub dtype: c_int,
+    pub rope_dims: c_int,
+    pub rope_interleaved: c_int,
+    pub rope_base: f64,
+    pub rope_freq: *const f64,
+}
+
+/// `nne_kv_append`.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct nne_kv_append {
+    pub q: *const f32,
+    pub k: *const f32,
+    pub v: *const f32,
+    pub q_out: *mut f32,
+    pub q_stride: usize,
+    pub k_stride: usize,
+    pub v_stride: usize,
+    pub tokens: usize,
+    pub q_heads: c_int,
+    pub eps: f32,
+    pub q_gamma: *const f32,
+    pub k_gamma: *const f32,
+    pub page_table: *const i32,
+    pub table_stride: usize,
+    pub sequences: c_int,
+    pub sequence: *const i32,
+    pub index: *const i32,
+    pub position: *const i32,
+}
+
 pub const NNE_OK: c_int = 0;
 pub const NNE_ERR_INVALID_ARGUMENT: c_int = 1;
 pub const NNE_ERR_SHAPE_MISMATCH: c_int = 2;
@@ -49,6 +94,8 @@ pub const NNE_ERR_UNSUPPORTED: c_int = 7;
 pub const NNE_INPUT_PLAIN: c_int = 0;
 pub const NNE_INPUT_RMSNORM: c_int = 1;
 pub const NNE_INPUT_SILU_MUL: c_int = 2;
+pub const NNE_F16: c_int = 1;
+pub const NNE_BF16: c_int = 2;
 pub const NNE_SHARD_HANDLE_BYTES: usize = 64;
 
 extern "C" {
@@ -334,6 +381,23 @@ extern "C" {
         k: usize,
         y_dev: *mut f32,
         ldy: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn nne_kv_cache_create(
+        ctx: *mut nne_ctx,
+        desc: *const nne_kv_cache_desc,
+        out: *mut *mut nne_kv_cache,
+    ) -> c_int;
+    pub fn nne_kv_cache_destroy(cache: *mut nne_kv_cache) -> c_int;
+    pub fn nne_kv_cache_info(
+        cache: *const nne_kv_cache,
+        k_pages: *mut *mut c_void,
+        v_pages: *mut *mut c_void,
+        bytes_each: *mut usize,
+    ) -> c_int;
+    pub fn nne_kv_append_dev(
+        cache: *mut nne_kv_cache,
+        args: *const nne_kv_append,
         stream: *mut c_void,
     ) -> c_int;
     pub fn nne_shard_group_create(

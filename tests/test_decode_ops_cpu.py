@@ -14,3 +14,11 @@ def test_qlinear4_refusals_without_a_device(nne):
         nne.QLinear4.from_fields(np.zeros((2, 4), np.uint8), np.ones((2, 1), np.float32), None, 8, 2, 16)
     with pytest.raises(nne.InvalidArgument):
         nne.QLinear4.from_fields(np.zeros((2, 3), np.uint8), np.ones((2, 1), np.float32), None, 8, 2, 32)
+
+
+def test_cache_refusals_without_a_device(nne):
+    lib = nne.load()
+    assert lib.nne_kv_cache_create(None, None, None) == 1
+    assert lib.nne_kv_append_dev(None, None, None) == 1
+    assert lib.nne_kv_cache_info(None, None, None, None) == 1
+    assert lib.nne_kv_cache_destroy(None) == 0
