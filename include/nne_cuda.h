@@ -408,6 +408,39 @@ typedef struct nne_kv_append {
 } nne_kv_append;
 NNE_API int nne_kv_append_dev(nne_kv_cache *cache, const nne_kv_append *args, void *stream);
 
+/* Attention of the cache's newest tokens, drafted as a tree (or, one node a sequence, ordinary decoding): the
+ * attention call of src/models/llama.rs between the projections, over pages.  Sequence b has the rows
+ * node_start[b] .. node_start[b+1]-1 of q and out (node_start: [sequences + 1], ascending; rows outside are not
+ * touched), context[b] earlier tokens in places 0 .. context[b]-1 of the cache, which every node sees, and
+ * node j's key in place context[b] + j.  Node i sees node j where bit j of visible[row of i] is set - its ancestors
+ * and itself, as a rule - or, visible NULL, where j <= i (a chain); bits of nodes that are not there mean nothing.
+ *     out[row, h] = softmax(scale * q[row, h] . k) v      over what the node sees, head h / (q_heads / kv_heads)
+ * A row that sees nothing is 0.  What a row does not see does not reach it, Inf and NaN included.  Keys
+ * whose place the table does not name, or in a page outside the pool, are seen by nobody.  q and out are f32,
+ * [row][q_heads][head_dim] with a stride in floats from row to row, and do not overlap.  The products are of f32 accuracy (q
+ * and the probabilities keep 22 bits or more).  max_nodes (at most 64) bounds the nodes of a sequence: rows
+ * of a sequence beyond it are not written; longer chains go through in pieces of 64, appended piece by piece.
+ * max_context only guides how far the work is split; contexts may be longer.  One launch, no workspace,
+ * asynchronous on `stream`; results do not change from run to run. */
+typedef struct nne_tree_attention {
+    const float *q;
+    float *out;
+    size_t q_stride;
+    size_t out_stride;
+    size_t tokens;               /* rows of q and out */
+    int q_heads;
+    int sequences;
+    int max_nodes;
+    int max_context;
+    float scale;
+    const int32_t *node_start;
+    const int32_t *context;
+    const uint64_t *visible;
+    const int32_t *page_table;   /* [sequences][table_stride] */
+    size_t table_stride;
+} nne_tree_attention;
+NNE_API int nne_tree_attention_dev(nne_kv_cache *cache, const nne_tree_attention *args, void *stream);
+
 /* ---- column shards over the GPUs of one node -------------------------------------------------
  * The reference has no multi-device code.  Its forward computes output channel j from row j of
  * qweight, scales[j] and bias[j] alone (src/nn/quantized.rs:184-192) and quantizes per row

@@ -103,6 +103,7 @@ SIGNATURES = {
     "nne_kv_cache_destroy": (C.c_int, [C.c_void_p]),
     "nne_kv_cache_info": (C.c_int, [C.c_void_p, c_void_pp, c_void_pp, C.POINTER(C.c_size_t)]),
     "nne_kv_append_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nne_tree_attention_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "nne_shard_group_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, c_void_pp]),
     "nne_shard_group_handle": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nne_shard_group_connect": (C.c_int, [C.c_void_p, C.c_void_p]),
@@ -141,6 +142,14 @@ class KvAppendArgs(C.Structure):
                 ("eps", C.c_float), ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p), ("page_table", C.c_void_p),
                 ("table_stride", C.c_size_t), ("sequences", C.c_int), ("sequence", C.c_void_p), ("index", C.c_void_p),
                 ("position", C.c_void_p)]
+
+
+class TreeAttentionArgs(C.Structure):
+    """nne_tree_attention of include/nne_cuda.h."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_size_t), ("out_stride", C.c_size_t),
+                ("tokens", C.c_size_t), ("q_heads", C.c_int), ("sequences", C.c_int), ("max_nodes", C.c_int),
+                ("max_context", C.c_int), ("scale", C.c_float), ("node_start", C.c_void_p), ("context", C.c_void_p),
+                ("visible", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_size_t)]
 
 
 INPUT_PLAIN, INPUT_RMSNORM, INPUT_SILU_MUL = 0, 1, 2

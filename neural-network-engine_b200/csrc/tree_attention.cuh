@@ -1,0 +1,586 @@
+// Attention of drafted token trees over the paged cache: the kernel.  tree_attention.cu has the host side, and one
+// source file a cache type instantiates it.
+//
+// A row is one query head of one node.  The rows that share a key/value head - all nodes of a sequence times the
+// query heads of the group - meet each key together.  The scores are formed as S^T = K Q^T: mma.sync m16n8k16 with 16
+// keys on the M side and 8 rows on the N side, so that one node of a grouped head (4 or 8 rows) fills a tile that the
+// other way round would leave half empty; O^T = V^T P^T takes the probabilities back in by an 8x8 transpose in
+// registers (movmatrix).  Keys and values are the MMA's operands as they lie in the cache, exact.  q and P are f32: they
+// enter as sums of two (f16) or three (bf16) numbers of the cache's type, 22 or 24 bits, after a power of two
+// that keeps the small parts above f16's subnormals.  One part instead would be 2 to 3 times fewer MMAs and an error of 2^-11 or 2^-8
+// where the rest of the decode step keeps 2^-23.  A tile's products with P are summed from zero and join O by an f32 FMA that also
+// takes the rescaling by exp2(old max - new max): the running sum rounds once a tile, to nearest (the MMA truncates).
+//
+// One CTA takes up to 64 rows and a share of the keys in tiles of 64, double or triple buffered with
+// cp.async (rows of a tile come from up to eight pages); its warps split the tile's keys and the rows.  The
+// CTAs of a cluster take the shares of one set of rows and join max, sum and O through each other's shared memory, in rank
+// order: no workspace, no second launch, results that do not change from run to run.
+#pragma once
+
+#include "kvcache.cuh"
+#include "ptx.cuh"
+
+namespace nne {
+
+struct TreeArgs {
+    const float *q;
+    float *out;
+    size_t q_stride, out_stride;
+    int group, kv_heads;      // query heads of a key/value head
+    int tokens, max_nodes;
+    const int32_t *node_start, *context;
+    const uint64_t *visible;  // or null: a chain
+    const int32_t *page_table;
+    size_t table_stride, pages;
+    int page_shift;
+    float scale;              // times log2(e)
+    const void *k, *v;
+    int vec_out;
+};
+
+constexpr int TREE_KEYS = 64;   // keys of a tile
+constexpr int TREE_IDS = 8;     // tiles whose row numbers are held
+
+template <typename T>
+struct TreeType;
+template <>
+struct TreeType<__half> {
+    static constexpr int PARTS = 2;
+    static constexpr float P_BIAS = 15.0f;  // P is held times 2^15: its second part stays above the subnormals
+};
+template <>
+struct TreeType<__nv_bfloat16> {
+    static constexpr int PARTS = 3;
+    static constexpr float P_BIAS = 0.0f;
+};
+
+// NT: 8-row tiles of a warp; WN, WK: warps side by side along rows and along a tile's keys.
+template <typename T, int D, int NT, int WN, int WK>
+struct TreeShape {
+    static constexpr int PARTS = TreeType<T>::PARTS;
+    static constexpr int THREADS = WN * WK * 32;
+    static constexpr int ROWS = 8 * NT * WN;
+    static constexpr int KM = TREE_KEYS / (16 * WK);        // 16-key tiles of a warp
+    static constexpr int PITCH = 2 * D + 16;                // bytes of a key in shared memory: ldmatrix without conflicts
+    static constexpr int TILE = TREE_KEYS * PITCH;
+    static constexpr int STAGES = D <= 64 ? 4 : (D <= 128 && ROWS <= 8 ? 3 : 2);
+    static constexpr int Q_BYTES = PARTS * (ROWS / 8) * (D / 16) * 256;
+    static constexpr int OPITCH = D + 4;                    // floats of a row of O at the end
+    static constexpr int RING = STAGES * 2 * TILE;
+    static constexpr int O_BYTES = ROWS * OPITCH * 4;
+    static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;
+    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + (2 * WK + 2) * ROWS * 4 + TREE_IDS * TREE_KEYS * 4 + 16;
+    static constexpr int PER_SM = 2 * (SMEM + 1024) <= 227 * 1024 ? 2 : 1;
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes into shared memory, or zeros.
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t at, uint32_t rank) {
+    uint32_t peer;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t at, uint32_t rank) {
+    uint32_t peer;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int D, int NT, int WN, int WK>
+__global__ void __launch_bounds__(TreeShape<T, D, NT, WN, WK>::THREADS, TreeShape<T, D, NT, WN, WK>::PER_SM)
+tree_attention_kernel(const TreeArgs p) {
+    using S = TreeShape<T, D, NT, WN, WK>;
+    constexpr int PARTS = S::PARTS, KM = S::KM, ROWS = S::ROWS, THREADS = S::THREADS, STAGES = S::STAGES;
+    constexpr float NEG = -INFINITY;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint2 *qfrag = reinterpret_cast<uint2 *>(smem + S::MAIN);                     // [part][8-row tile][step][lane]
+    uint64_t *vis = reinterpret_cast<uint64_t *>(smem + S::MAIN + S::Q_BYTES);    // [ROWS]
+    float *qfac = reinterpret_cast<float *>(vis + ROWS);                          // [ROWS]
+    float *m_w = qfac + ROWS, *l_w = m_w + WK * ROWS;                             // [WK][ROWS] each
+    float *m_row = l_w + WK * ROWS, *l_row = m_row + ROWS;                        // [ROWS] each
+    int *ids = reinterpret_cast<int *>(l_row + ROWS);                             // [TREE_IDS][TREE_KEYS]
+    unsigned long long *odd_keys = reinterpret_cast<unsigned long long *>(
+        (reinterpret_cast<uintptr_t>(ids + TREE_IDS * TREE_KEYS) + 7) & ~(uintptr_t)7);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int wn = warp % WN, wk = warp / WN, g = lane >> 2, t4 = lane & 3;
+    const unsigned split = gridDim.x, rank = blockIdx.x;
+    const int kvh = blockIdx.y % p.kv_heads, b = blockIdx.z;
+    const int row_base = (int)(blockIdx.y / p.kv_heads) * ROWS;
+
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    const int start = p.node_start[b];
+    int nodes = p.node_start[b + 1] - start;
+    nodes = start < 0 || start > p.tokens ? 0 : min(min(nodes, p.max_nodes), p.tokens - start);
+    const int rows = max(nodes, 0) * p.group;
+    if (row_base >= rows) return;  // the whole cluster
+    const int nrows = min(ROWS, rows - row_base);
+    const int ctx = max(p.context[b], 0);
+    const long long room = (long long)p.table_stride << p.page_shift;  // places that the table can name
+    const int total = (int)min((long long)ctx + nodes, min(room, 0x7fffffc0ll));
+    const int tiles = (total + TREE_KEYS - 1) / TREE_KEYS;
+    const int per = (tiles + (int)split - 1) / (int)split;
+    const int t0 = min((int)rank * per, tiles), t1 = min(t0 + per, tiles);
+    const int32_t *table = p.page_table + (size_t)b * p.table_stride;
+
+    // Row of the pool for this thread's key of a tile (-1: none).
+    auto id_of = [&](int tile) {
+        const int key = tile * TREE_KEYS + tid;
+        return key < total ? kv_row(table, p.table_stride, key, p.page_shift, p.pages, p.kv_heads, kvh) : -1;
+    };
+    const uint32_t ring = smem_u32(smem);
+    auto issue = [&](int tile) {
+        if (tile < t1) {
+            const int *id = ids + (tile % TREE_IDS) * TREE_KEYS;
+            const uint32_t dst = ring + ((tile - t0) % STAGES) * 2 * S::TILE;
+#pragma unroll 4
+            for (int i = tid; i < TREE_KEYS * (D / 8); i += THREADS) {
+                const int r = i / (D / 8), c = i % (D / 8), row = id[r];
+                const size_t at = ((size_t)(row < 0 ? 0 : row) * D + c * 8) * 2;
+                cp_async_16_or_zero(dst + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.k) + at, row >= 0);
+                cp_async_16_or_zero(dst + S::TILE + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.v) + at, row >= 0);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (tid < TREE_KEYS) {
+#pragma unroll
+        for (int j = 0; j < STAGES; ++j)
+            if (t0 + j < t1) ids[((t0 + j) % TREE_IDS) * TREE_KEYS + tid] = id_of(t0 + j);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < STAGES - 1; ++j) issue(t0 + j);
+
+    // Queries: scale * log2(e) * q, as parts of the cache's type in the MMA's operand order.  f16: times a power of two
+    // that brings a row's largest to [2^13, 2^14).
+    for (int r = warp; r < ROWS; r += THREADS / 32) {
+        constexpr int PL = (D / 2 + 31) / 32;  // pairs of a lane
+        float2 x[PL];
+        float top = 0.0f;
+        const int row = row_base + r, node = row / p.group;
+        const bool there = r < nrows;
+        const float *src = p.q + (size_t)(there ? start + node : 0) * p.q_stride + (size_t)(kvh * p.group + row % p.group) * D;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int c = lane + i * 32;
+            x[i] = make_float2(0.0f, 0.0f);
+            if (there && c < D / 2) x[i] = make_float2(src[2 * c] * p.scale, src[2 * c + 1] * p.scale);
+            top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+        }
+        float up = 1.0f, down = 1.0f;
+        if (sizeof(T) == 2 && PARTS == 2) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            int e = 13 + 127 - ((int)(__float_as_uint(top) >> 23) & 255);
+            e = e > 120 ? 120 : (e < -114 ? -114 : e);
+            up = __uint_as_float((uint32_t)(e + 127) << 23);
+            down = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int c = lane + i * 32;
+            if (c >= D / 2) continue;
+            float2 v = make_float2(x[i].x * up, x[i].y * up);
+            const int step = c / 8, word = (c % 8) / 4, at = (r % 8) * 4 + c % 4;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                const uint32_t w = pack_pair<T>(v.x, v.y);
+                const float2 back = unpack_pair<T>(w);
+                v = make_float2(v.x - back.x, v.y - back.y);
+                reinterpret_cast<uint32_t *>(qfrag + ((q * (ROWS / 8) + r / 8) * (D / 16) + step) * 32 + at)[word] = w;
+            }
+        }
+        if (lane == 0) {
+            qfac[r] = down;
+            uint64_t bits = 0;
+            if (there) bits = p.visible ? p.visible[start + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
+            vis[r] = bits;
+        }
+    }
+
+    float o[D / 16][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = NEG, l[n][0] = l[n][1] = 0.0f;
+
+    for (int t = t0; t < t1; ++t) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncthreads();  // tile t is there for everybody; tile t - 1's buffer is free
+        issue(t + STAGES - 1);
+        int next_id = -1;  // looked up now, stored below: the table's latency passes under the tile's work
+        const bool looks = tid < TREE_KEYS && t + STAGES < t1;
+        if (looks) next_id = id_of(t + STAGES);
+        const uint32_t kt = ring + ((t - t0) % STAGES) * 2 * S::TILE, vt = kt + S::TILE;
+        const int *id = ids + (t % TREE_IDS) * TREE_KEYS;
+        const int key0 = t * TREE_KEYS;
+        const bool drafted = key0 + TREE_KEYS > ctx;  // the tile holds keys that not every node sees (or none)
+
+        // A drafted key that some row does not see must not reach it through 0 * Inf or 0 * NaN: values that are not
+        // finite are taken out of the tile and added by hand to the rows that see them.
+        unsigned long long odd = 0;
+        if (drafted) {
+            if (tid == 0) *odd_keys = 0;
+            __syncthreads();
+            for (int i = tid; i < TREE_KEYS * (D / 8); i += THREADS) {
+                const int r = i / (D / 8), c = i % (D / 8);
+                if (key0 + r < ctx || key0 + r >= total) continue;
+                const uint4 w = *reinterpret_cast<const uint4 *>(smem + (vt - ring) + r * S::PITCH + c * 16);
+                const uint32_t e = PARTS == 2 ? 0x7c00u : 0x7f80u;
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                bool bad = false;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) bad |= (x[q] & e) == e || ((x[q] >> 16) & e) == e;
+                if (bad) atomicOr(odd_keys, 1ull << r);
+            }
+            __syncthreads();
+            odd = *odd_keys;
+            if (odd) {  // the same for the whole CTA
+                for (int i = tid; i < TREE_KEYS * (D / 8); i += THREADS) {
+                    const int r = i / (D / 8), c = i % (D / 8);
+                    if (odd >> r & 1) *reinterpret_cast<uint4 *>(smem + (vt - ring) + r * S::PITCH + c * 16) = make_uint4(0, 0, 0, 0);
+                }
+                __syncthreads();
+            }
+        }
+
+        if (wn * 8 * NT < nrows) {  // a warp without rows only helps to load
+            // S^T: the small parts of q in one accumulator, the large one in another
+            float s[KM][NT][4], s2[KM][NT][4];
+#pragma unroll
+            for (int k = 0; k < KM; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[k][n][e] = s2[k][n][e] = 0.0f;
+            const uint32_t ka = kt + (wk * KM * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
+            const uint2 *qf = qfrag + (wn * NT) * (D / 16) * 32 + lane;
+#pragma unroll
+            for (int step = 0; step < D / 16; ++step) {
+                uint32_t a[KM][4];
+#pragma unroll
+                for (int k = 0; k < KM; ++k) ldsm_x4(a[k], ka + k * 16 * S::PITCH + step * 32);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) {
+                        const uint2 w = qf[((q * (ROWS / 8) + n) * (D / 16) + step) * 32];
+#pragma unroll
+                        for (int k = 0; k < KM; ++k) {
+                            if (q == 0) mma_16x8x16<T>(s[k][n], a[k], w.x, w.y);
+                            else mma_16x8x16<T>(s2[k][n], a[k], w.x, w.y);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float f0 = PARTS == 2 ? qfac[(wn * NT + n) * 8 + 2 * t4] : 1.0f;
+                const float f1 = PARTS == 2 ? qfac[(wn * NT + n) * 8 + 2 * t4 + 1] : 1.0f;
+#pragma unroll
+                for (int k = 0; k < KM; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[k][n][e] = (s[k][n][e] + s2[k][n][e]) * ((e & 1) ? f1 : f0);
+            }
+            // What a row does not see, and keys without a place in the pool.
+            bool gap = false;
+#pragma unroll
+            for (int k = 0; k < KM; ++k) gap |= id[(wk * KM + k) * 16 + (lane & 15)] < 0;
+            if (drafted || __any_sync(0xffffffffu, gap)) {
+#pragma unroll
+                for (int k = 0; k < KM; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = (wk * KM + k) * 16 + h * 8 + g, j = key0 + r - ctx;
+                        const bool there = id[r] >= 0;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const bool sees = there && (j < 0 || (vis[(wn * NT + n) * 8 + 2 * t4 + e] >> j & 1));
+                                if (!sees) s[k][n][2 * h + e] = NEG;
+                            }
+                    }
+            }
+            // Running maximum, probabilities, their sum.
+            float alpha[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = m[n][e];
+#pragma unroll
+                    for (int k = 0; k < KM; ++k) top = fmaxf(top, fmaxf(s[k][n][e], s[k][n][2 + e]));
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                    const float ref = top == NEG ? 0.0f : top;
+                    alpha[n][e] = exp2f(m[n][e] - ref);
+                    m[n][e] = top;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < KM; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float v = exp2f(s[k][n][2 * h + e] - ref + TreeType<T>::P_BIAS);
+                            s[k][n][2 * h + e] = v;
+                            sum += v;
+                        }
+                    l[n][e] = fmaf(l[n][e], alpha[n][e], sum);
+                }
+            // P^T in parts, transposed into operand order, the smallest part first.
+            uint32_t pf[KM][NT][PARTS][2];
+#pragma unroll
+            for (int k = 0; k < KM; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float2 v = make_float2(s[k][n][2 * h], s[k][n][2 * h + 1]);
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q) {
+                            const uint32_t w = pack_pair<T>(v.x, v.y);
+                            const float2 back = unpack_pair<T>(w);
+                            v = make_float2(v.x - back.x, v.y - back.y);
+                            pf[k][n][PARTS - 1 - q][h] = transpose_8x8(w);
+                        }
+                    }
+            const uint32_t va = vt + (wk * KM * 16 + (lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                float add[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) add[n][0] = add[n][1] = add[n][2] = add[n][3] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KM; ++k) {
+                    uint32_t a[4];
+                    ldsm_x4_trans(a, va + k * 16 * S::PITCH + i * 32);
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[n], a, pf[k][n][q][0], pf[k][n][q][1]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], add[n][e]);
+            }
+            if (odd) {
+                const T *vg = static_cast<const T *>(p.v);
+#pragma unroll
+                for (int k = 0; k < KM; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = (wk * KM + k) * 16 + h * 8 + j;
+                            if (!(odd >> r & 1)) continue;
+                            const size_t at = (size_t)max(id[r], 0) * D;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float w = __shfl_sync(0xffffffffu, s[k][n][2 * h + e], j * 4 + t4);
+                                    if (w == 0.0f) continue;
+#pragma unroll
+                                    for (int i = 0; i < D / 16; ++i) {
+                                        o[i][n][e] += w * (float)vg[at + i * 16 + g];
+                                        o[i][n][2 + e] += w * (float)vg[at + i * 16 + 8 + g];
+                                    }
+                                }
+                        }
+            }
+        }
+        if (looks) ids[((t + STAGES) % TREE_IDS) * TREE_KEYS + tid] = next_id;
+    }
+
+    // The warps along the keys join: maximum and sum of a row, then O, warp after warp.
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+            if (g == 0) {
+                const int r = (wn * NT + n) * 8 + 2 * t4 + e;
+                m_w[wk * ROWS + r] = m[n][e];
+                l_w[wk * ROWS + r] = l[n][e];
+            }
+        }
+    __syncthreads();
+    float *om = reinterpret_cast<float *>(smem);
+    float f[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = (wn * NT + n) * 8 + 2 * t4 + e;
+            float top = NEG, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, m_w[w * ROWS + r]);
+            const float ref = top == NEG ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) sum += l_w[w * ROWS + r] * exp2f(m_w[w * ROWS + r] - ref);
+            f[n][e] = exp2f(m[n][e] - ref);
+            if (wk == 0 && g == 0) m_row[r] = top, l_row[r] = sum;
+        }
+    for (int w = 0; w < WK; ++w) {
+        if (wk == w) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float *at = om + ((wn * NT + n) * 8 + 2 * t4 + (e & 1)) * S::OPITCH + i * 16 + (e >> 1) * 8 + g;
+                        const float v = o[i][n][e] * f[n][e & 1];
+                        *at = w == 0 ? v : *at + v;
+                    }
+        }
+        __syncthreads();
+    }
+
+    // The CTAs of the cluster join, rank after rank; each writes its share of the rows' elements.
+    if (split > 1) cluster_meet();
+    const uint32_t om_at = smem_u32(om), m_at = smem_u32(m_row), l_at = smem_u32(l_row);
+    for (int i = (int)rank * THREADS + tid; i < nrows * (D / 4); i += (int)split * THREADS) {
+        const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+        float top = NEG;
+        for (unsigned w = 0; w < split; ++w) top = fmaxf(top, ld_cluster_f32(m_at + r * 4, w));
+        const float ref = top == NEG ? 0.0f : top;
+        float sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (unsigned w = 0; w < split; ++w) {
+            const float k = exp2f(ld_cluster_f32(m_at + r * 4, w) - ref);
+            const float4 x = ld_cluster_f4(om_at + (r * S::OPITCH + c) * 4, w);
+            sum = fmaf(ld_cluster_f32(l_at + r * 4, w), k, sum);
+            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y), v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
+        }
+        if (sum == 0.0f) {
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a row that sees nothing
+        } else {
+            v.x = __fdiv_rn(v.x, sum), v.y = __fdiv_rn(v.y, sum), v.z = __fdiv_rn(v.z, sum), v.w = __fdiv_rn(v.w, sum);
+        }
+        const int row = row_base + r;
+        float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D + c;
+        if (p.vec_out) {
+            *reinterpret_cast<float4 *>(dst) = v;
+        } else {
+            dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+        }
+    }
+    if (split > 1) cluster_meet();  // nobody leaves while a peer may still read its shared memory
+}
+
+template <typename T, int D, int NT, int WN, int WK>
+int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
+    using S = TreeShape<T, D, NT, WN, WK>;
+    auto kernel = tree_attention_kernel<T, D, NT, WN, WK>;
+    const size_t blocks = (size_t)a.kv_heads * ((max_rows + S::ROWS - 1) / S::ROWS);
+    if (blocks > 65535 || sequences > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "too many heads or sequences for one launch");
+    NNE_TRY(ensure_dynamic_smem(ctx->device, kernel, S::SMEM));
+    // Split the keys while that fills SMs that would have no CTA and a share keeps two tiles.  Powers of two up to
+    // 16: any of them finds a place in the GPU's clusters.
+    const size_t slots = (size_t)ctx->sm_count * S::PER_SM, have = blocks * sequences;
+    const long long tiles = (max_keys + TREE_KEYS - 1) / TREE_KEYS;
+    unsigned split = 1;
+    while (split < 16 && have * split * 2 <= slots && tiles >= (long long)split * 4) split *= 2;
+    if (split > 8) {  // clusters of 16 are asked for once a device
+        static std::atomic<uint64_t> asked{0};
+        const uint64_t bit = 1ull << (ctx->device & 63);
+        if (!(asked.load(std::memory_order_acquire) & bit)) {
+            NNE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            asked.fetch_or(bit, std::memory_order_release);
+        }
+    }
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split, (unsigned)blocks, (unsigned)sequences);
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    count_launch();
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(NNE_ERR_CUDA, "tree attention launch failed: %s", cudaGetErrorString(e));
+    }
+    return NNE_OK;
+}
+
+// Shapes by the rows a key/value head meets at most: the fewest idle MMA columns.  O takes D/16 * NT * 4 registers a
+// thread, so heads of 256 keep to one 8-row tile a warp.
+template <typename T, int D>
+int launch_tree_d(nne_ctx *ctx, const TreeArgs &a, int sequences, long long max_keys, cudaStream_t s) {
+    const int rows = a.max_nodes * a.group;
+    if (rows <= 8) return launch_tree_shape<T, D, 1, 1, 4>(ctx, a, sequences, rows, max_keys, s);
+    if constexpr (D <= 128) {
+        if (rows <= 16) return launch_tree_shape<T, D, 2, 1, 4>(ctx, a, sequences, rows, max_keys, s);
+        if (rows <= 32) return launch_tree_shape<T, D, 2, 2, 2>(ctx, a, sequences, rows, max_keys, s);
+        return launch_tree_shape<T, D, 2, 4, 2>(ctx, a, sequences, rows, max_keys, s);
+    } else {
+        if (rows <= 16) return launch_tree_shape<T, D, 1, 2, 2>(ctx, a, sequences, rows, max_keys, s);
+        return launch_tree_shape<T, D, 1, 4, 2>(ctx, a, sequences, rows, max_keys, s);
+    }
+}
+
+template <typename T>
+int launch_tree(nne_ctx *ctx, int d, const TreeArgs &a, int sequences, long long max_keys, cudaStream_t s) {
+    switch (d) {
+        case 64: return launch_tree_d<T, 64>(ctx, a, sequences, max_keys, s);
+        case 96: return launch_tree_d<T, 96>(ctx, a, sequences, max_keys, s);
+        case 128: return launch_tree_d<T, 128>(ctx, a, sequences, max_keys, s);
+        default: return launch_tree_d<T, 256>(ctx, a, sequences, max_keys, s);
+    }
+}
+int launch_tree_f16(nne_ctx *ctx, int d, const TreeArgs &a, int sequences, long long max_keys, cudaStream_t s);
+int launch_tree_bf16(nne_ctx *ctx, int d, const TreeArgs &a, int sequences, long long max_keys, cudaStream_t s);
+
+}  // namespace nne

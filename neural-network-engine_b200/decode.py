@@ -94,3 +94,23 @@ class KvAppend(_Call):
 
     def run(self, stream: int = 0) -> None:
         self._issue(self.cache.handle, stream)
+
+
+class TreeAttention(_Call):
+    """Attention of the newest tokens of each sequence over the cache (``nne_tree_attention_dev``): a tree of up to 64
+    drafted nodes, a chain (``visible`` 0) or, one node a sequence, ordinary decoding.  ``node_start`` i32
+    ``[sequences + 1]``, ``context`` i32 ``[sequences]``, ``visible`` u64 ``[tokens]``; ``scale`` defaults to
+    ``head_dim ** -0.5``."""
+
+    def __init__(self, cache: PagedKvCache, tokens: int, q_heads: int, q: int, out: int, sequences: int, node_start: int, context: int,
+                 page_table: int, table_stride: int, max_nodes: int, max_context: int, visible: int = 0, scale: Optional[float] = None,
+                 q_stride: int = 0, out_stride: int = 0):
+        width = q_heads * cache.head_dim
+        super().__init__(load().nne_tree_attention_dev, _lib.TreeAttentionArgs(
+            q or None, out or None, q_stride or width, out_stride or width, tokens, q_heads, sequences, max_nodes, max_context,
+            cache.head_dim ** -0.5 if scale is None else scale, node_start or None, context or None, visible or None,
+            page_table or None, table_stride))
+        self.cache = cache
+
+    def run(self, stream: int = 0) -> None:
+        self._issue(self.cache.handle, stream)

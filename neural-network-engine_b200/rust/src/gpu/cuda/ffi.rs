@@ -83,6 +83,27 @@ pub struct nne_kv_append {
     pub position: *const i32,
 }
 
+/// `nne_tree_attention`.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct nne_tree_attention {
+    pub q: *const f32,
+    pub out: *mut f32,
+    pub q_stride: usize,
+    pub out_stride: usize,
+    pub tokens: usize,
+    pub q_heads: c_int,
+    pub sequences: c_int,
+    pub max_nodes: c_int,
+    pub max_context: c_int,
+    pub scale: f32,
+    pub node_start: *const i32,
+    pub context: *const i32,
+    pub visible: *const u64,
+    pub page_table: *const i32,
+    pub table_stride: usize,
+}
+
 pub const NNE_OK: c_int = 0;
 pub const NNE_ERR_INVALID_ARGUMENT: c_int = 1;
 pub const NNE_ERR_SHAPE_MISMATCH: c_int = 2;
@@ -398,6 +419,11 @@ extern "C" {
     pub fn nne_kv_append_dev(
         cache: *mut nne_kv_cache,
         args: *const nne_kv_append,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn nne_tree_attention_dev(
+        cache: *mut nne_kv_cache,
+        args: *const nne_tree_attention,
         stream: *mut c_void,
     ) -> c_int;
     pub fn nne_shard_group_create(

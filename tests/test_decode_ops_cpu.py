@@ -22,3 +22,7 @@ def test_cache_refusals_without_a_device(nne):
     assert lib.nne_kv_append_dev(None, None, None) == 1
     assert lib.nne_kv_cache_info(None, None, None, None) == 1
     assert lib.nne_kv_cache_destroy(None) == 0
+
+
+def test_attention_refusals_without_a_device(nne):
+    assert nne.load().nne_tree_attention_dev(None, None, None) == 1
