@@ -441,6 +441,34 @@ typedef struct nne_tree_attention {
 } nne_tree_attention;
 NNE_API int nne_tree_attention_dev(nne_kv_cache *cache, const nne_tree_attention *args, void *stream);
 
+/* ---- the next token --------------------------------------------------------------------------------
+ * One token a row from logits [rows][vocab] f32 (a stride in floats from row to row; what the output projection
+ * leaves, src/models/llama.rs), by settings of each row's own; every settings pointer is to [rows] device numbers
+ * or NULL for "off":
+ *     w_i = exp((l_i - max l) / temperature)      NULL: 1; a temperature that is not above 0 takes the argmax
+ *     top_k > 0: only the first k in the order "larger logit first, of equal ones the lower index"
+ *     top_p < 1: of those only the shortest prefix of that order whose mass reaches top_p * (their mass); at
+ *                least one
+ *     min_p > 0: of those only w_i >= min_p (the largest w is 1; above 1 counts as 1)
+ *     token   = the first index, in index order, at which the mass kept so far exceeds uniform * (mass kept)
+ * uniform[row] is in [0, 1).  NaN logits count as -inf, which is never drawn; -0 equals 0; a row without any other
+ * logit gives -1.  Masses are held in units of 2^-40 of the largest weight: the draw is that of exact arithmetic but where
+ * uniform lies within about 1e-7 of a border.  The same inputs give the same tokens.  vocab is at most 2^22.
+ * One launch, no workspace, asynchronous on `stream`. */
+typedef struct nne_sample {
+    const float *logits;
+    size_t row_stride;
+    size_t rows;
+    size_t vocab;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+    const float *uniform;
+    int32_t *tokens;
+} nne_sample;
+NNE_API int nne_sample_dev(nne_ctx *ctx, const nne_sample *args, void *stream);
+
 /* ---- column shards over the GPUs of one node -------------------------------------------------
  * The reference has no multi-device code.  Its forward computes output channel j from row j of
  * qweight, scales[j] and bias[j] alone (src/nn/quantized.rs:184-192) and quantizes per row

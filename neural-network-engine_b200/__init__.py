@@ -23,7 +23,7 @@ from .quantized import (  # noqa: F401
     rmsnorm_device,
     silu_mul_device,
 )
-from .decode import KvAppend, PagedKvCache, TreeAttention  # noqa: F401
+from .decode import KvAppend, PagedKvCache, Sampler, TreeAttention  # noqa: F401
 from .quantized4 import QLinear4, quantize_rows4_device  # noqa: F401
 from . import safetensors_int8  # noqa: F401
 from .safetensors_int8 import load_qlinear, save_qlinears  # noqa: F401

@@ -104,6 +104,7 @@ SIGNATURES = {
     "nne_kv_cache_info": (C.c_int, [C.c_void_p, c_void_pp, c_void_pp, C.POINTER(C.c_size_t)]),
     "nne_kv_append_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "nne_tree_attention_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nne_sample_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "nne_shard_group_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, c_void_pp]),
     "nne_shard_group_handle": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nne_shard_group_connect": (C.c_int, [C.c_void_p, C.c_void_p]),
@@ -150,6 +151,13 @@ class TreeAttentionArgs(C.Structure):
                 ("tokens", C.c_size_t), ("q_heads", C.c_int), ("sequences", C.c_int), ("max_nodes", C.c_int),
                 ("max_context", C.c_int), ("scale", C.c_float), ("node_start", C.c_void_p), ("context", C.c_void_p),
                 ("visible", C.c_void_p), ("page_table", C.c_void_p), ("table_stride", C.c_size_t)]
+
+
+class SampleArgs(C.Structure):
+    """nne_sample of include/nne_cuda.h."""
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_size_t), ("rows", C.c_size_t), ("vocab", C.c_size_t),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("uniform", C.c_void_p), ("tokens", C.c_void_p)]
 
 
 INPUT_PLAIN, INPUT_RMSNORM, INPUT_SILU_MUL = 0, 1, 2

@@ -114,3 +114,18 @@ class TreeAttention(_Call):
 
     def run(self, stream: int = 0) -> None:
         self._issue(self.cache.handle, stream)
+
+
+class Sampler(_Call):
+    """One token a row of logits, from given uniform numbers (``nne_sample_dev``).  ``temperature``, ``top_k`` (i32),
+    ``top_p`` and ``min_p`` are addresses of one setting a row, 0 for "off"; ``tokens`` i32 ``[rows]``."""
+
+    def __init__(self, ctx: CudaContext, rows: int, vocab: int, logits: int, uniform: int, tokens: int, temperature: int = 0,
+                 top_k: int = 0, top_p: int = 0, min_p: int = 0, row_stride: int = 0):
+        super().__init__(load().nne_sample_dev, _lib.SampleArgs(
+            logits or None, row_stride or vocab, rows, vocab, temperature or None, top_k or None, top_p or None, min_p or None,
+            uniform or None, tokens or None))
+        self.ctx = ctx
+
+    def run(self, stream: int = 0) -> None:
+        self._issue(self.ctx.handle, stream)

@@ -104,6 +104,22 @@ pub struct nne_tree_attention {
     pub table_stride: usize,
 }
 
+/// `nne_sample`.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct nne_sample {
+    pub logits: *const f32,
+    pub row_stride: usize,
+    pub rows: usize,
+    pub vocab: usize,
+    pub temperature: *const f32,
+    pub top_k: *const i32,
+    pub top_p: *const f32,
+    pub min_p: *const f32,
+    pub uniform: *const f32,
+    pub tokens: *mut i32,
+}
+
 pub const NNE_OK: c_int = 0;
 pub const NNE_ERR_INVALID_ARGUMENT: c_int = 1;
 pub const NNE_ERR_SHAPE_MISMATCH: c_int = 2;
@@ -426,6 +442,7 @@ extern "C" {
         args: *const nne_tree_attention,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn nne_sample_dev(ctx: *mut nne_ctx, args: *const nne_sample, stream: *mut c_void) -> c_int;
     pub fn nne_shard_group_create(
         ctx: *mut nne_ctx,
         rank: c_int,

@@ -26,3 +26,7 @@ def test_cache_refusals_without_a_device(nne):
 
 def test_attention_refusals_without_a_device(nne):
     assert nne.load().nne_tree_attention_dev(None, None, None) == 1
+
+
+def test_sampling_refusals_without_a_device(nne):
+    assert nne.load().nne_sample_dev(None, None, None) == 1
