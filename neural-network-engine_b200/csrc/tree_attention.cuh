@@ -63,7 +63,7 @@ struct TreeShape {
     static constexpr int KM = TREE_KEYS / (16 * WK);        // 16-key tiles of a warp
     static constexpr int PITCH = 2 * D + 16;                // bytes of a key in shared memory: ldmatrix without conflicts
     static constexpr int TILE = TREE_KEYS * PITCH;
-    static constexpr int STAGES = D <= 64 ? 4 : (D <= 128 && ROWS <= 8 ? 3 : 2);
+    static constexpr int STAGES = D <= 64 ? 4 : 2;
     static constexpr int Q_BYTES = PARTS * (ROWS / 8) * (D / 16) * 256;
     static constexpr int OPITCH = D + 4;                    // floats of a row of O at the end
     static constexpr int RING = STAGES * 2 * TILE;
@@ -83,22 +83,25 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 template <typename T>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // 16 bytes into shared memory, or zeros.
 __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void *src, bool there) {
@@ -120,6 +123,147 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t at, uint32_t rank) {
 }
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Queries: scale * log2(e) * q, as parts of the cache's type in the MMA's operand order [part][8-row tile][step][lane].
+// f16: times a power of two that brings a row's largest to [2^13, 2^14), undone by qfac.  vis: what a row's node sees.
+template <typename T, int D, int ROWS, int THREADS>
+__device__ __forceinline__ void tree_queries(const TreeArgs &p, uint2 *qfrag, uint64_t *vis, float *qfac, int start, int row_base, int nrows, int kvh) {
+    constexpr int PARTS = TreeType<T>::PARTS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = warp; r < ROWS; r += THREADS / 32) {
+        constexpr int PL = (D / 2 + 31) / 32;  // pairs of a lane
+        float2 x[PL];
+        float top = 0.0f;
+        const int row = row_base + r, node = row / p.group;
+        const bool there = r < nrows;
+        const float *src = p.q + (size_t)(there ? start + node : 0) * p.q_stride + (size_t)(kvh * p.group + row % p.group) * D;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int c = lane + i * 32;
+            x[i] = make_float2(0.0f, 0.0f);
+            if (there && c < D / 2) x[i] = make_float2(src[2 * c] * p.scale, src[2 * c + 1] * p.scale);
+            top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+        }
+        float up = 1.0f, down = 1.0f;
+        if (sizeof(T) == 2 && PARTS == 2) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            int e = 13 + 127 - ((int)(__float_as_uint(top) >> 23) & 255);
+            e = e > 120 ? 120 : (e < -114 ? -114 : e);
+            up = __uint_as_float((uint32_t)(e + 127) << 23);
+            down = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int c = lane + i * 32;
+            if (c >= D / 2) continue;
+            float2 v = make_float2(x[i].x * up, x[i].y * up);
+            const int step = c / 8, word = (c % 8) / 4, at = (r % 8) * 4 + c % 4;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                const uint32_t w = pack_pair<T>(v.x, v.y);
+                const float2 back = unpack_pair<T>(w);
+                v = make_float2(v.x - back.x, v.y - back.y);
+                reinterpret_cast<uint32_t *>(qfrag + ((q * (ROWS / 8) + r / 8) * (D / 16) + step) * 32 + at)[word] = w;
+            }
+        }
+        if (lane == 0) {
+            qfac[r] = down;
+            uint64_t bits = 0;
+            if (there) bits = p.visible ? p.visible[start + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
+            vis[r] = bits;
+        }
+    }
+}
+
+// Joins what the warps along the keys and the CTAs of the cluster have of each row, and writes the rows.  o: 16 dimensions x 8
+// rows a tile as the MMA leaves them; m, l: maximum and (this lane's part of the) sum.  `smem`: ROWS * (D + 4) floats.
+template <int D, int NT, int WN, int WK>
+__device__ __forceinline__ void tree_join(const TreeArgs &p, const float (&o)[D / 16][NT][4], const float (&m)[NT][2], float (&l)[NT][2], uint8_t *smem,
+                                          float *m_w, float *l_w, float *m_row, float *l_row, int start, int row_base, int nrows, int kvh) {
+    constexpr int ROWS = 8 * NT * WN, THREADS = WN * WK * 32, OPITCH = D + 4;
+    constexpr float NEG = -INFINITY;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int wn = warp % WN, wk = warp / WN, g = lane >> 2, t4 = lane & 3;
+    const unsigned split = gridDim.x, rank = blockIdx.x;
+    // The warps along the keys join: maximum and sum of a row, then O, warp after warp.
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+            if (g == 0) {
+                const int r = (wn * NT + n) * 8 + 2 * t4 + e;
+                m_w[wk * ROWS + r] = m[n][e];
+                l_w[wk * ROWS + r] = l[n][e];
+            }
+        }
+    __syncthreads();
+    float *om = reinterpret_cast<float *>(smem);
+    float f[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = (wn * NT + n) * 8 + 2 * t4 + e;
+            float top = NEG, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, m_w[w * ROWS + r]);
+            const float ref = top == NEG ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) sum += l_w[w * ROWS + r] * exp2f(m_w[w * ROWS + r] - ref);
+            f[n][e] = exp2f(m[n][e] - ref);
+            if (wk == 0 && g == 0) m_row[r] = top, l_row[r] = sum;
+        }
+    for (int w = 0; w < WK; ++w) {
+        if (wk == w) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float *at = om + ((wn * NT + n) * 8 + 2 * t4 + (e & 1)) * OPITCH + i * 16 + (e >> 1) * 8 + g;
+                        const float v = o[i][n][e] * f[n][e & 1];
+                        *at = w == 0 ? v : *at + v;
+                    }
+        }
+        __syncthreads();
+    }
+
+    // The CTAs of the cluster join, rank after rank; each writes its share of the rows' elements.
+    if (split > 1) cluster_meet();
+    const uint32_t om_at = smem_u32(om), m_at = smem_u32(m_row), l_at = smem_u32(l_row);
+    for (int i = (int)rank * THREADS + tid; i < nrows * (D / 4); i += (int)split * THREADS) {
+        const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+        float top = NEG;
+        for (unsigned w = 0; w < split; ++w) top = fmaxf(top, ld_cluster_f32(m_at + r * 4, w));
+        const float ref = top == NEG ? 0.0f : top;
+        float sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (unsigned w = 0; w < split; ++w) {
+            const float k = exp2f(ld_cluster_f32(m_at + r * 4, w) - ref);
+            const float4 x = ld_cluster_f4(om_at + (r * OPITCH + c) * 4, w);
+            sum = fmaf(ld_cluster_f32(l_at + r * 4, w), k, sum);
+            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y), v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
+        }
+        if (sum == 0.0f) {
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a row that sees nothing
+        } else {
+            v.x = __fdiv_rn(v.x, sum), v.y = __fdiv_rn(v.y, sum), v.z = __fdiv_rn(v.z, sum), v.w = __fdiv_rn(v.w, sum);
+        }
+        const int row = row_base + r;
+        float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D + c;
+        if (p.vec_out) {
+            *reinterpret_cast<float4 *>(dst) = v;
+        } else {
+            dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+        }
+    }
+    if (split > 1) cluster_meet();  // nobody leaves while a peer may still read its shared memory
 }
 
 template <typename T, int D, int NT, int WN, int WK>
@@ -189,52 +333,7 @@ tree_attention_kernel(const TreeArgs p) {
 #pragma unroll
     for (int j = 0; j < STAGES - 1; ++j) issue(t0 + j);
 
-    // Queries: scale * log2(e) * q, as parts of the cache's type in the MMA's operand order.  f16: times a power of two
-    // that brings a row's largest to [2^13, 2^14).
-    for (int r = warp; r < ROWS; r += THREADS / 32) {
-        constexpr int PL = (D / 2 + 31) / 32;  // pairs of a lane
-        float2 x[PL];
-        float top = 0.0f;
-        const int row = row_base + r, node = row / p.group;
-        const bool there = r < nrows;
-        const float *src = p.q + (size_t)(there ? start + node : 0) * p.q_stride + (size_t)(kvh * p.group + row % p.group) * D;
-#pragma unroll
-        for (int i = 0; i < PL; ++i) {
-            const int c = lane + i * 32;
-            x[i] = make_float2(0.0f, 0.0f);
-            if (there && c < D / 2) x[i] = make_float2(src[2 * c] * p.scale, src[2 * c + 1] * p.scale);
-            top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
-        }
-        float up = 1.0f, down = 1.0f;
-        if (sizeof(T) == 2 && PARTS == 2) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            int e = 13 + 127 - ((int)(__float_as_uint(top) >> 23) & 255);
-            e = e > 120 ? 120 : (e < -114 ? -114 : e);
-            up = __uint_as_float((uint32_t)(e + 127) << 23);
-            down = __uint_as_float((uint32_t)(127 - e) << 23);
-        }
-#pragma unroll
-        for (int i = 0; i < PL; ++i) {
-            const int c = lane + i * 32;
-            if (c >= D / 2) continue;
-            float2 v = make_float2(x[i].x * up, x[i].y * up);
-            const int step = c / 8, word = (c % 8) / 4, at = (r % 8) * 4 + c % 4;
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-                const uint32_t w = pack_pair<T>(v.x, v.y);
-                const float2 back = unpack_pair<T>(w);
-                v = make_float2(v.x - back.x, v.y - back.y);
-                reinterpret_cast<uint32_t *>(qfrag + ((q * (ROWS / 8) + r / 8) * (D / 16) + step) * 32 + at)[word] = w;
-            }
-        }
-        if (lane == 0) {
-            qfac[r] = down;
-            uint64_t bits = 0;
-            if (there) bits = p.visible ? p.visible[start + node] : (node >= 63 ? ~0ull : (2ull << node) - 1);
-            vis[r] = bits;
-        }
-    }
+    tree_queries<T, D, ROWS, THREADS>(p, qfrag, vis, qfac, start, row_base, nrows, kvh);
 
     float o[D / 16][NT][4];
     float m[NT][2], l[NT][2];
@@ -302,9 +401,9 @@ tree_attention_kernel(const TreeArgs p) {
 #pragma unroll
                 for (int k = 0; k < KM; ++k) ldsm_x4(a[k], ka + k * 16 * S::PITCH + step * 32);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) {
+                    for (int n = 0; n < NT; ++n) {
                         const uint2 w = qf[((q * (ROWS / 8) + n) * (D / 16) + step) * 32];
 #pragma unroll
                         for (int k = 0; k < KM; ++k) {
@@ -385,24 +484,32 @@ tree_attention_kernel(const TreeArgs p) {
                         }
                     }
             const uint32_t va = vt + (wk * KM * 16 + (lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+            constexpr int W = 2;  // dimension tiles side by side: no MMA waits for the one before it
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                float add[NT][4];
+            for (int i = 0; i < D / 16; i += W) {
+                float add[W][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) add[n][0] = add[n][1] = add[n][2] = add[n][3] = 0.0f;
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) add[w][n][0] = add[w][n][1] = add[w][n][2] = add[w][n][3] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KM; ++k) {
-                    uint32_t a[4];
-                    ldsm_x4_trans(a, va + k * 16 * S::PITCH + i * 32);
+                    uint32_t a[W][4];
+#pragma unroll
+                    for (int w = 0; w < W; ++w) ldsm_x4_trans(a[w], va + k * 16 * S::PITCH + (i + w) * 32);
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[n], a, pf[k][n][q][0], pf[k][n][q][1]);
+                        for (int w = 0; w < W; ++w)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[w][n], a[w], pf[k][n][q][0], pf[k][n][q][1]);
                 }
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int w = 0; w < W; ++w)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], add[n][e]);
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i + w][n][e] = fmaf(o[i + w][n][e], alpha[n][e & 1], add[w][n][e]);
             }
             if (odd) {
                 const T *vg = static_cast<const T *>(p.v);
@@ -432,100 +539,311 @@ tree_attention_kernel(const TreeArgs p) {
         if (looks) ids[((t + STAGES) % TREE_IDS) * TREE_KEYS + tid] = next_id;
     }
 
-    // The warps along the keys join: maximum and sum of a row, then O, warp after warp.
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    tree_join<D, NT, WN, WK>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
+}
+
+// Few rows (one node, or a few of a small group): the keys are all the work.  Each of the CTA's four warps takes every
+// fourth group of 16 keys of the share and loads it for itself, so that no warp ever waits for another: with tiles shared by the CTA a
+// tile of 64 keys took 1950 cycles, most of them at barriers and in address arithmetic.  Eight keys in a row lie in one page (pages are
+// 8 places or more), so a group is two look-ups, made one group ahead of the copies they serve.
+template <typename T, int D, int NT>
+struct DecodeShape {
+    static constexpr int PARTS = TreeType<T>::PARTS;
+    static constexpr int ROWS = 8 * NT, THREADS = 128;
+    static constexpr int PITCH = 2 * D + 16;
+    static constexpr int HALF = 16 * PITCH;                 // 16 keys; a slot is keys and values
+    static constexpr int SLOTS = D <= 64 ? 5 : 3;
+    static constexpr int RING = 4 * SLOTS * 2 * HALF;
+    static constexpr int O_BYTES = ROWS * (D + 4) * 4;
+    static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;
+    static constexpr int Q_BYTES = PARTS * NT * (D / 16) * 256;
+    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + 10 * ROWS * 4 + 4 * SLOTS * 2 * 4;
+    static constexpr int PER_SM = 2 * (SMEM + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr bool Q_REGS = NT * (D / 16) * PARTS * 2 <= 48;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128, DecodeShape<T, D, NT>::PER_SM) tree_decode_kernel(const TreeArgs p) {
+    using S = DecodeShape<T, D, NT>;
+    constexpr int PARTS = S::PARTS, ROWS = S::ROWS, SLOTS = S::SLOTS;
+    constexpr float NEG = -INFINITY;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint2 *qfrag = reinterpret_cast<uint2 *>(smem + S::MAIN);
+    uint64_t *vis = reinterpret_cast<uint64_t *>(smem + S::MAIN + S::Q_BYTES);
+    float *qfac = reinterpret_cast<float *>(vis + ROWS);
+    float *m_w = qfac + ROWS, *l_w = m_w + 4 * ROWS, *m_row = l_w + 4 * ROWS, *l_row = m_row + ROWS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    int *ids = reinterpret_cast<int *>(l_row + ROWS) + warp * SLOTS * 2;  // [slot][2]: rows of the pool of the group's halves
+    const int kvh = blockIdx.y % p.kv_heads, b = blockIdx.z;
+    const int row_base = (int)(blockIdx.y / p.kv_heads) * ROWS;
+
+    grid_dependency_wait();
+    grid_launch_dependents();
+
+    const int start = p.node_start[b];
+    int nodes = p.node_start[b + 1] - start;
+    nodes = start < 0 || start > p.tokens ? 0 : min(min(nodes, p.max_nodes), p.tokens - start);
+    const int rows = max(nodes, 0) * p.group;
+    if (row_base >= rows) return;  // the whole cluster
+    const int nrows = min(ROWS, rows - row_base);
+    const int ctx = max(p.context[b], 0);
+    const long long room = (long long)p.table_stride << p.page_shift;
+    const int total = (int)min((long long)ctx + nodes, min(room, 0x7fffffc0ll));
+    const int groups = (total + 15) / 16, per = (groups + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int g0 = min((int)blockIdx.x * per, groups) + warp, g1 = min((int)blockIdx.x * per + per, groups);
+    const int32_t *table = p.page_table + (size_t)b * p.table_stride;
+
+    // Row of the pool of half `lane` (0, 1) of a group, or -1.
+    auto look = [&](int grp) {
+        const int key = grp * 16 + lane * 8;
+        return lane < 2 && grp < g1 && key < total ? kv_row(table, p.table_stride, key, p.page_shift, p.pages, p.kv_heads, kvh) : -1;
+    };
+    const uint32_t ring = smem_u32(smem) + warp * (SLOTS * 2 * S::HALF);
+    auto issue = [&](int grp, int slot, int row) {
+        if (grp < g1) {
+            const int r0 = __shfl_sync(0xffffffffu, row, 0), r1 = __shfl_sync(0xffffffffu, row, 1);
+            if (lane < 2) ids[slot * 2 + lane] = row;
+            const int left = total - grp * 16;
+            const uint32_t dst = ring + slot * 2 * S::HALF;
+            if (left >= 16 && r0 >= 0 && r1 >= 0) {
+                const uint8_t *k0 = static_cast<const uint8_t *>(p.k) + (size_t)r0 * D * 2, *k1 = static_cast<const uint8_t *>(p.k) + ((size_t)r1 - 8) * D * 2;
+                const ptrdiff_t to_v = static_cast<const uint8_t *>(p.v) - static_cast<const uint8_t *>(p.k);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
-            if (g == 0) {
-                const int r = (wn * NT + n) * 8 + 2 * t4 + e;
-                m_w[wk * ROWS + r] = m[n][e];
-                l_w[wk * ROWS + r] = l[n][e];
+                for (int j = 0; j < D / 16; ++j) {
+                    const int i = lane + 32 * j, r = i / (D / 8), c = i % (D / 8);
+                    const uint8_t *src = (r < 8 ? k0 : k1) + (r * D + c * 8) * 2;
+                    cp_async_16(dst + r * S::PITCH + c * 16, src);
+                    cp_async_16(dst + S::HALF + r * S::PITCH + c * 16, src + to_v);
+                }
+            } else {
+                for (int j = 0; j < D / 16; ++j) {
+                    const int i = lane + 32 * j, r = i / (D / 8), c = i % (D / 8), base = r < 8 ? r0 : r1;
+                    const bool there = r < left && base >= 0;
+                    const size_t at = ((size_t)(there ? base + (r & 7) : 0) * D + c * 8) * 2;
+                    cp_async_16_or_zero(dst + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.k) + at, there);
+                    cp_async_16_or_zero(dst + S::HALF + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.v) + at, there);
+                }
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    {
+        int row[SLOTS];
+#pragma unroll
+        for (int j = 0; j < SLOTS - 1; ++j) row[j] = look(g0 + 4 * j);
+#pragma unroll
+        for (int j = 0; j < SLOTS - 1; ++j) issue(g0 + 4 * j, j, row[j]);
+    }
+    int next = look(g0 + 4 * (SLOTS - 1));
+
+    tree_queries<T, D, ROWS, 128>(p, qfrag, vis, qfac, start, row_base, nrows, kvh);
     __syncthreads();
-    float *om = reinterpret_cast<float *>(smem);
-    float f[NT][2];
+    uint2 qr[S::Q_REGS ? NT * (D / 16) * PARTS : 1];
+    if constexpr (S::Q_REGS) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < NT * (D / 16) * PARTS; ++i) qr[i] = qfrag[i * 32 + lane];
+    }
+    float qf[NT][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = (wn * NT + n) * 8 + 2 * t4 + e;
-            float top = NEG, sum = 0.0f;
+    for (int n = 0; n < NT; ++n) qf[n][0] = qfac[n * 8 + 2 * t4], qf[n][1] = qfac[n * 8 + 2 * t4 + 1];
+
+    float o[D / 16][NT][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, m_w[w * ROWS + r]);
-            const float ref = top == NEG ? 0.0f : top;
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int w = 0; w < WK; ++w) sum += l_w[w * ROWS + r] * exp2f(m_w[w * ROWS + r] - ref);
-            f[n][e] = exp2f(m[n][e] - ref);
-            if (wk == 0 && g == 0) m_row[r] = top, l_row[r] = sum;
+        for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = NEG, l[n][0] = l[n][1] = 0.0f;
+
+    int slot = 0;
+    for (int grp = g0; grp < g1; grp += 4) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
+        __syncwarp();  // the group is there for every lane, and every lane is done with the slot before
+        issue(grp + 4 * (SLOTS - 1), slot == 0 ? SLOTS - 1 : slot - 1, next);
+        next = look(grp + 4 * SLOTS);
+        const uint32_t kt = ring + slot * 2 * S::HALF, vt = kt + S::HALF;
+        const int key0 = grp * 16;
+        const bool drafted = key0 + 16 > ctx;
+
+        // Values of drafted keys that are not finite leave the slot and are added by hand to the rows that see them:
+        // 0 * Inf must not reach the others.
+        unsigned odd = 0;
+        if (drafted) {
+            for (int i = lane; i < 16 * (D / 8); i += 32) {
+                const int r = i / (D / 8), c = i % (D / 8);
+                if (key0 + r < ctx || key0 + r >= total) continue;
+                const uint4 w = *reinterpret_cast<const uint4 *>(smem + (vt - smem_u32(smem)) + r * S::PITCH + c * 16);
+                const uint32_t e = PARTS == 2 ? 0x7c00u : 0x7f80u;
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if ((x[q] & e) == e || ((x[q] >> 16) & e) == e) odd |= 1u << r;
+            }
+            odd = __reduce_or_sync(0xffffffffu, odd);
+            if (odd) {
+                for (int i = lane; i < 16 * (D / 8); i += 32) {
+                    const int r = i / (D / 8), c = i % (D / 8);
+                    if (odd >> r & 1) *reinterpret_cast<uint4 *>(smem + (vt - smem_u32(smem)) + r * S::PITCH + c * 16) = make_uint4(0, 0, 0, 0);
+                }
+                __syncwarp();
+            }
         }
-    for (int w = 0; w < WK; ++w) {
-        if (wk == w) {
+
+        // S^T, in chains of their own for each part and, one tile of rows, for even and odd steps: an MMA waits for
+        // the one before it in its chain
+        constexpr int CH = NT == 1 ? 2 : 1;
+        float s[NT][4], sp[CH][PARTS][NT][4];
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sp[c][q][n][0] = sp[c][q][n][1] = sp[c][q][n][2] = sp[c][q][n][3] = 0.0f;
+        const uint32_t ka = kt + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
+#pragma unroll
+        for (int step = 0; step < D / 16; ++step) {
+            uint32_t a[4];
+            ldsm_x4(a, ka + step * 32);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int at = (q * NT + n) * (D / 16) + step;
+                    uint2 w;
+                    if constexpr (S::Q_REGS) w = qr[at];
+                    else w = qfrag[at * 32 + lane];
+                    mma_16x8x16<T>(sp[step % CH][q][n], a, w.x, w.y);
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float v = 0.0f;
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) v += sp[c][q][n][e];
+                s[n][e] = PARTS == 2 ? v * qf[n][e & 1] : v;
+            }
+        const int id0 = ids[slot * 2], id1 = ids[slot * 2 + 1];
+        if (drafted || id0 < 0 || id1 < 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = h * 8 + g, j = key0 + r - ctx;
+                const bool there = (h ? id1 : id0) >= 0 && key0 + r < total;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float *at = om + ((wn * NT + n) * 8 + 2 * t4 + (e & 1)) * S::OPITCH + i * 16 + (e >> 1) * 8 + g;
-                        const float v = o[i][n][e] * f[n][e & 1];
-                        *at = w == 0 ? v : *at + v;
+                    for (int e = 0; e < 2; ++e) {
+                        const bool sees = there && (j < 0 || (vis[n * 8 + 2 * t4 + e] >> j & 1));
+                        if (!sees) s[n][2 * h + e] = NEG;
                     }
+            }
         }
-        __syncthreads();
+        float alpha[NT][2];
+        uint32_t pf[NT][PARTS][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float top = fmaxf(m[n][e], fmaxf(s[n][e], s[n][2 + e]));
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                const float ref = top == NEG ? 0.0f : top;
+                alpha[n][e] = exp2f(m[n][e] - ref);
+                m[n][e] = top;
+                s[n][e] = exp2f(s[n][e] - ref + TreeType<T>::P_BIAS);
+                s[n][2 + e] = exp2f(s[n][2 + e] - ref + TreeType<T>::P_BIAS);
+                l[n][e] = fmaf(l[n][e], alpha[n][e], s[n][e] + s[n][2 + e]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float2 v = make_float2(s[n][2 * h], s[n][2 * h + 1]);
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    const uint32_t w = pack_pair<T>(v.x, v.y);
+                    const float2 back = unpack_pair<T>(w);
+                    v = make_float2(v.x - back.x, v.y - back.y);
+                    pf[n][PARTS - 1 - q][h] = transpose_8x8(w);
+                }
+            }
+        }
+        const uint32_t va = vt + ((lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16;
+        constexpr int W = NT == 1 ? (D % 64 ? 2 : 4) : 2;  // dimension tiles side by side
+#pragma unroll
+        for (int i = 0; i < D / 16; i += W) {
+            uint32_t a[W][4];
+            float add[W][NT][4];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                ldsm_x4_trans(a[w], va + (i + w) * 32);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) add[w][n][0] = add[w][n][1] = add[w][n][2] = add[w][n][3] = 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[w][n], a[w], pf[n][q][0], pf[n][q][1]);
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i + w][n][e] = fmaf(o[i + w][n][e], alpha[n][e & 1], add[w][n][e]);
+        }
+        if (odd) {
+            const T *vg = static_cast<const T *>(p.v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                for (int j = 0; j < 8; ++j) {
+                    if (!(odd >> (h * 8 + j) & 1)) continue;
+                    const size_t at = (size_t)(max(h ? id1 : id0, 0) + j) * D;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float w = __shfl_sync(0xffffffffu, s[n][2 * h + e], j * 4 + t4);
+                            if (w == 0.0f) continue;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) {
+                                o[i][n][e] += w * (float)vg[at + i * 16 + g];
+                                o[i][n][2 + e] += w * (float)vg[at + i * 16 + 8 + g];
+                            }
+                        }
+                }
+        }
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
-
-    // The CTAs of the cluster join, rank after rank; each writes its share of the rows' elements.
-    if (split > 1) cluster_meet();
-    const uint32_t om_at = smem_u32(om), m_at = smem_u32(m_row), l_at = smem_u32(l_row);
-    for (int i = (int)rank * THREADS + tid; i < nrows * (D / 4); i += (int)split * THREADS) {
-        const int r = i / (D / 4), c = (i % (D / 4)) * 4;
-        float top = NEG;
-        for (unsigned w = 0; w < split; ++w) top = fmaxf(top, ld_cluster_f32(m_at + r * 4, w));
-        const float ref = top == NEG ? 0.0f : top;
-        float sum = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (unsigned w = 0; w < split; ++w) {
-            const float k = exp2f(ld_cluster_f32(m_at + r * 4, w) - ref);
-            const float4 x = ld_cluster_f4(om_at + (r * S::OPITCH + c) * 4, w);
-            sum = fmaf(ld_cluster_f32(l_at + r * 4, w), k, sum);
-            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y), v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
-        }
-        if (sum == 0.0f) {
-            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a row that sees nothing
-        } else {
-            v.x = __fdiv_rn(v.x, sum), v.y = __fdiv_rn(v.y, sum), v.z = __fdiv_rn(v.z, sum), v.w = __fdiv_rn(v.w, sum);
-        }
-        const int row = row_base + r;
-        float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D + c;
-        if (p.vec_out) {
-            *reinterpret_cast<float4 *>(dst) = v;
-        } else {
-            dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
-        }
-    }
-    if (split > 1) cluster_meet();  // nobody leaves while a peer may still read its shared memory
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the ring is done with: O goes over it
+    tree_join<D, NT, 1, 4>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
 }
 
-template <typename T, int D, int NT, int WN, int WK>
-int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
-    using S = TreeShape<T, D, NT, WN, WK>;
-    auto kernel = tree_attention_kernel<T, D, NT, WN, WK>;
-    const size_t blocks = (size_t)a.kv_heads * ((max_rows + S::ROWS - 1) / S::ROWS);
+// Into how many CTAs (of a cluster) the keys of one set of rows go.  A CTA's time is its keys and, in their measure, about 256
+// for starting, queries and the join; CTAs run in rounds of `slots`.  Sizes the GPU's clusters take; 16 needs asking for.
+inline unsigned tree_split(size_t have, size_t slots, long long keys) {
+    unsigned best = 1;
+    double least = 1e300;
+    for (unsigned s : {1u, 2u, 3u, 4u, 6u, 8u, 16u}) {
+        if (s > 1 && keys < (long long)s * 2 * TREE_KEYS) break;
+        const double cost = (double)((have * s + slots - 1) / slots) * ((double)keys / s + 256.0);
+        if (cost < least * 0.98) best = s, least = cost;
+    }
+    return best;
+}
+
+template <typename K>
+int launch_tree_kernel(nne_ctx *ctx, K kernel, std::atomic<uint64_t> &asked, int threads, size_t smem, int per_sm, int rows_of_cta, const TreeArgs &a,
+                       int sequences, int max_rows, long long max_keys, cudaStream_t s) {
+    const size_t blocks = (size_t)a.kv_heads * ((max_rows + rows_of_cta - 1) / rows_of_cta);
     if (blocks > 65535 || sequences > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "too many heads or sequences for one launch");
-    NNE_TRY(ensure_dynamic_smem(ctx->device, kernel, S::SMEM));
-    // Split the keys while that fills SMs that would have no CTA and a share keeps two tiles.  Powers of two up to
-    // 16: any of them finds a place in the GPU's clusters.
-    const size_t slots = (size_t)ctx->sm_count * S::PER_SM, have = blocks * sequences;
-    const long long tiles = (max_keys + TREE_KEYS - 1) / TREE_KEYS;
-    unsigned split = 1;
-    while (split < 16 && have * split * 2 <= slots && tiles >= (long long)split * 4) split *= 2;
+    NNE_TRY(ensure_dynamic_smem(ctx->device, kernel, smem));
+    const unsigned split = tree_split(blocks * sequences, (size_t)ctx->sm_count * per_sm, max_keys);
     if (split > 8) {  // clusters of 16 are asked for once a device
-        static std::atomic<uint64_t> asked{0};
         const uint64_t bit = 1ull << (ctx->device & 63);
         if (!(asked.load(std::memory_order_acquire) & bit)) {
             NNE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -541,8 +859,8 @@ int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_ro
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(split, (unsigned)blocks, (unsigned)sequences);
-    cfg.blockDim = dim3(S::THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -555,14 +873,28 @@ int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_ro
     return NNE_OK;
 }
 
+template <typename T, int D, int NT>
+int launch_decode(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
+    using S = DecodeShape<T, D, NT>;
+    static std::atomic<uint64_t> asked{0};
+    return launch_tree_kernel(ctx, tree_decode_kernel<T, D, NT>, asked, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, a, sequences, max_rows, max_keys, s);
+}
+template <typename T, int D, int NT, int WN, int WK>
+int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
+    using S = TreeShape<T, D, NT, WN, WK>;
+    static std::atomic<uint64_t> asked{0};
+    return launch_tree_kernel(ctx, tree_attention_kernel<T, D, NT, WN, WK>, asked, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, a, sequences, max_rows,
+                              max_keys, s);
+}
+
 // Shapes by the rows a key/value head meets at most: the fewest idle MMA columns.  O takes D/16 * NT * 4 registers a
 // thread, so heads of 256 keep to one 8-row tile a warp.
 template <typename T, int D>
 int launch_tree_d(nne_ctx *ctx, const TreeArgs &a, int sequences, long long max_keys, cudaStream_t s) {
     const int rows = a.max_nodes * a.group;
-    if (rows <= 8) return launch_tree_shape<T, D, 1, 1, 4>(ctx, a, sequences, rows, max_keys, s);
+    if (rows <= 8) return launch_decode<T, D, 1>(ctx, a, sequences, rows, max_keys, s);
     if constexpr (D <= 128) {
-        if (rows <= 16) return launch_tree_shape<T, D, 2, 1, 4>(ctx, a, sequences, rows, max_keys, s);
+        if (rows <= 16) return launch_decode<T, D, 2>(ctx, a, sequences, rows, max_keys, s);
         if (rows <= 32) return launch_tree_shape<T, D, 2, 2, 2>(ctx, a, sequences, rows, max_keys, s);
         return launch_tree_shape<T, D, 2, 4, 2>(ctx, a, sequences, rows, max_keys, s);
     } else {
