@@ -420,8 +420,9 @@ NNE_API int nne_kv_append_dev(nne_kv_cache *cache, const nne_kv_append *args, vo
  * [row][q_heads][head_dim] with a stride in floats from row to row, and do not overlap.  The products are of f32 accuracy (q
  * and the probabilities keep 22 bits or more).  max_nodes (at most 64) bounds the nodes of a sequence: rows
  * of a sequence beyond it are not written; longer chains go through in pieces of 64, appended piece by piece.
- * max_context only guides how far the work is split; contexts may be longer.  One launch, no workspace,
- * asynchronous on `stream`; results do not change from run to run. */
+ * max_context only guides how far the work is split; contexts may be longer.  One launch without workspace, or, few rows
+ * over long contexts, two with a stream-ordered workspace of at most a few megabytes; asynchronous on `stream`.  Results
+ * do not change from run to run. */
 typedef struct nne_tree_attention {
     const float *q;
     float *out;

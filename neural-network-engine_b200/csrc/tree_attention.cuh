@@ -36,6 +36,9 @@ struct TreeArgs {
     float scale;              // times log2(e)
     const void *k, *v;
     int vec_out;
+    // Shares that a cluster cannot hold: each CTA leaves its rows here, [set of rows][share][row][D + 4] with the maximum and
+    // the sum behind a row's D numbers, and tree_gather_kernel joins them.
+    float *part;
 };
 
 constexpr int TREE_KEYS = 64;   // keys of a tile
@@ -67,9 +70,9 @@ struct TreeShape {
     static constexpr int Q_BYTES = PARTS * (ROWS / 8) * (D / 16) * 256;
     static constexpr int OPITCH = D + 4;                    // floats of a row of O at the end
     static constexpr int RING = STAGES * 2 * TILE;
-    static constexpr int O_BYTES = ROWS * OPITCH * 4;
+    static constexpr int O_BYTES = WK * ROWS * OPITCH * 4;
     static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;
-    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + (2 * WK + 2) * ROWS * 4 + TREE_IDS * TREE_KEYS * 4 + 16;
+    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + (2 * WK + 2) * ROWS * 4 + TREE_IDS * (TREE_KEYS / 8) * 4 + 16;
     static constexpr int PER_SM = 2 * (SMEM + 1024) <= 227 * 1024 ? 2 : 1;
 };
 
@@ -178,7 +181,7 @@ __device__ __forceinline__ void tree_queries(const TreeArgs &p, uint2 *qfrag, ui
 }
 
 // Joins what the warps along the keys and the CTAs of the cluster have of each row, and writes the rows.  o: 16 dimensions x 8
-// rows a tile as the MMA leaves them; m, l: maximum and (this lane's part of the) sum.  `smem`: ROWS * (D + 4) floats.
+// rows a tile as the MMA leaves them; m, l: maximum and (this lane's part of the) sum.  `smem`: WK * ROWS * (D + 4) floats.
 template <int D, int NT, int WN, int WK>
 __device__ __forceinline__ void tree_join(const TreeArgs &p, const float (&o)[D / 16][NT][4], const float (&m)[NT][2], float (&l)[NT][2], uint8_t *smem,
                                           float *m_w, float *l_w, float *m_row, float *l_row, int start, int row_base, int nrows, int kvh) {
@@ -201,37 +204,43 @@ __device__ __forceinline__ void tree_join(const TreeArgs &p, const float (&o)[D 
                 l_w[wk * ROWS + r] = l[n][e];
             }
         }
+    __syncthreads();  // m, l; and nobody reads the ring any more: O goes over it
+    float *om = reinterpret_cast<float *>(smem);  // [WK][ROWS][OPITCH], the sum into the first
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                om[(wk * ROWS + (wn * NT + n) * 8 + 2 * t4 + (e & 1)) * OPITCH + i * 16 + (e >> 1) * 8 + g] = o[i][n][e];
     __syncthreads();
-    float *om = reinterpret_cast<float *>(smem);
-    float f[NT][2];
+    for (int i = tid; i < nrows * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+        float top = NEG, sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, m_w[w * ROWS + r]);
+        const float ref = top == NEG ? 0.0f : top;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = (wn * NT + n) * 8 + 2 * t4 + e;
-            float top = NEG, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, m_w[w * ROWS + r]);
-            const float ref = top == NEG ? 0.0f : top;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) sum += l_w[w * ROWS + r] * exp2f(m_w[w * ROWS + r] - ref);
-            f[n][e] = exp2f(m[n][e] - ref);
-            if (wk == 0 && g == 0) m_row[r] = top, l_row[r] = sum;
+        for (int w = 0; w < WK; ++w) {
+            const float k = exp2f(m_w[w * ROWS + r] - ref);
+            const float4 x = *reinterpret_cast<const float4 *>(om + (w * ROWS + r) * OPITCH + c);
+            sum = fmaf(l_w[w * ROWS + r], k, sum);
+            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y), v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
         }
-    for (int w = 0; w < WK; ++w) {
-        if (wk == w) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float *at = om + ((wn * NT + n) * 8 + 2 * t4 + (e & 1)) * OPITCH + i * 16 + (e >> 1) * 8 + g;
-                        const float v = o[i][n][e] * f[n][e & 1];
-                        *at = w == 0 ? v : *at + v;
-                    }
+        *reinterpret_cast<float4 *>(om + r * OPITCH + c) = v;
+        if (c == 0) m_row[r] = top, l_row[r] = sum;
+    }
+    __syncthreads();
+
+    if (p.part) {
+        float *mine = p.part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * split + rank) * ROWS * (D + 4);
+        for (int i = tid; i < nrows * (D / 4); i += THREADS) {
+            const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+            *reinterpret_cast<float4 *>(mine + r * (D + 4) + c) = *reinterpret_cast<const float4 *>(om + r * OPITCH + c);
+            if (c == 0) mine[r * (D + 4) + D] = m_row[r], mine[r * (D + 4) + D + 1] = l_row[r];
         }
-        __syncthreads();
+        return;
     }
 
     // The CTAs of the cluster join, rank after rank; each writes its share of the rows' elements.
@@ -278,9 +287,9 @@ tree_attention_kernel(const TreeArgs p) {
     float *qfac = reinterpret_cast<float *>(vis + ROWS);                          // [ROWS]
     float *m_w = qfac + ROWS, *l_w = m_w + WK * ROWS;                             // [WK][ROWS] each
     float *m_row = l_w + WK * ROWS, *l_row = m_row + ROWS;                        // [ROWS] each
-    int *ids = reinterpret_cast<int *>(l_row + ROWS);                             // [TREE_IDS][TREE_KEYS]
+    int *ids = reinterpret_cast<int *>(l_row + ROWS);                             // [TREE_IDS][TREE_KEYS / 8]
     unsigned long long *odd_keys = reinterpret_cast<unsigned long long *>(
-        (reinterpret_cast<uintptr_t>(ids + TREE_IDS * TREE_KEYS) + 7) & ~(uintptr_t)7);
+        (reinterpret_cast<uintptr_t>(ids + TREE_IDS * (TREE_KEYS / 8)) + 7) & ~(uintptr_t)7);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wn = warp % WN, wk = warp / WN, g = lane >> 2, t4 = lane & 3;
     const unsigned split = gridDim.x, rank = blockIdx.x;
@@ -304,30 +313,33 @@ tree_attention_kernel(const TreeArgs p) {
     const int t0 = min((int)rank * per, tiles), t1 = min(t0 + per, tiles);
     const int32_t *table = p.page_table + (size_t)b * p.table_stride;
 
-    // Row of the pool for this thread's key of a tile (-1: none).
+    // Row of the pool of eight keys of a tile (thread < 8), or -1: eight in a row lie in one page.
     auto id_of = [&](int tile) {
-        const int key = tile * TREE_KEYS + tid;
+        const int key = tile * TREE_KEYS + tid * 8;
         return key < total ? kv_row(table, p.table_stride, key, p.page_shift, p.pages, p.kv_heads, kvh) : -1;
     };
     const uint32_t ring = smem_u32(smem);
     auto issue = [&](int tile) {
         if (tile < t1) {
-            const int *id = ids + (tile % TREE_IDS) * TREE_KEYS;
+            const int *id = ids + (tile % TREE_IDS) * (TREE_KEYS / 8);
             const uint32_t dst = ring + ((tile - t0) % STAGES) * 2 * S::TILE;
-#pragma unroll 4
-            for (int i = tid; i < TREE_KEYS * (D / 8); i += THREADS) {
-                const int r = i / (D / 8), c = i % (D / 8), row = id[r];
-                const size_t at = ((size_t)(row < 0 ? 0 : row) * D + c * 8) * 2;
-                cp_async_16_or_zero(dst + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.k) + at, row >= 0);
-                cp_async_16_or_zero(dst + S::TILE + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.v) + at, row >= 0);
+            const int left = total - tile * TREE_KEYS;
+            static_assert(TREE_KEYS * (D / 8) % THREADS == 0, "whole rounds of copies");
+#pragma unroll
+            for (int j = 0; j < TREE_KEYS * (D / 8) / THREADS; ++j) {
+                const int i = tid + j * THREADS, r = i / (D / 8), c = i % (D / 8), row = id[r >> 3];
+                const bool there = row >= 0 && r < left;
+                const size_t at = ((size_t)(there ? row + (r & 7) : 0) * D + c * 8) * 2;
+                cp_async_16_or_zero(dst + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.k) + at, there);
+                cp_async_16_or_zero(dst + S::TILE + r * S::PITCH + c * 16, static_cast<const uint8_t *>(p.v) + at, there);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (tid < TREE_KEYS) {
+    if (tid < TREE_KEYS / 8) {
 #pragma unroll
         for (int j = 0; j < STAGES; ++j)
-            if (t0 + j < t1) ids[((t0 + j) % TREE_IDS) * TREE_KEYS + tid] = id_of(t0 + j);
+            if (t0 + j < t1) ids[((t0 + j) % TREE_IDS) * (TREE_KEYS / 8) + tid] = id_of(t0 + j);
     }
     __syncthreads();
 #pragma unroll
@@ -349,10 +361,10 @@ tree_attention_kernel(const TreeArgs p) {
         __syncthreads();  // tile t is there for everybody; tile t - 1's buffer is free
         issue(t + STAGES - 1);
         int next_id = -1;  // looked up now, stored below: the table's latency passes under the tile's work
-        const bool looks = tid < TREE_KEYS && t + STAGES < t1;
+        const bool looks = tid < TREE_KEYS / 8 && t + STAGES < t1;
         if (looks) next_id = id_of(t + STAGES);
         const uint32_t kt = ring + ((t - t0) % STAGES) * 2 * S::TILE, vt = kt + S::TILE;
-        const int *id = ids + (t % TREE_IDS) * TREE_KEYS;
+        const int *id = ids + (t % TREE_IDS) * (TREE_KEYS / 8);
         const int key0 = t * TREE_KEYS;
         const bool drafted = key0 + TREE_KEYS > ctx;  // the tile holds keys that not every node sees (or none)
 
@@ -424,14 +436,14 @@ tree_attention_kernel(const TreeArgs p) {
             // What a row does not see, and keys without a place in the pool.
             bool gap = false;
 #pragma unroll
-            for (int k = 0; k < KM; ++k) gap |= id[(wk * KM + k) * 16 + (lane & 15)] < 0;
+            for (int k = 0; k < KM; ++k) gap |= id[(wk * KM + k) * 2 + (lane & 1)] < 0;
             if (drafted || __any_sync(0xffffffffu, gap)) {
 #pragma unroll
                 for (int k = 0; k < KM; ++k)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int r = (wk * KM + k) * 16 + h * 8 + g, j = key0 + r - ctx;
-                        const bool there = id[r] >= 0;
+                        const bool there = id[r >> 3] >= 0 && key0 + r < total;
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -520,7 +532,7 @@ tree_attention_kernel(const TreeArgs p) {
                         for (int j = 0; j < 8; ++j) {
                             const int r = (wk * KM + k) * 16 + h * 8 + j;
                             if (!(odd >> r & 1)) continue;
-                            const size_t at = (size_t)max(id[r], 0) * D;
+                            const size_t at = (size_t)(max(id[r >> 3], 0) + (r & 7)) * D;
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -536,7 +548,7 @@ tree_attention_kernel(const TreeArgs p) {
                         }
             }
         }
-        if (looks) ids[((t + STAGES) % TREE_IDS) * TREE_KEYS + tid] = next_id;
+        if (looks) ids[((t + STAGES) % TREE_IDS) * (TREE_KEYS / 8) + tid] = next_id;
     }
 
     tree_join<D, NT, WN, WK>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
@@ -549,29 +561,30 @@ tree_attention_kernel(const TreeArgs p) {
 template <typename T, int D, int NT>
 struct DecodeShape {
     static constexpr int PARTS = TreeType<T>::PARTS;
-    static constexpr int ROWS = 8 * NT, THREADS = 128;
+    static constexpr int WARPS = 4;
+    static constexpr int ROWS = 8 * NT, THREADS = WARPS * 32;
     static constexpr int PITCH = 2 * D + 16;
     static constexpr int HALF = 16 * PITCH;                 // 16 keys; a slot is keys and values
     static constexpr int SLOTS = D <= 64 ? 5 : 3;
-    static constexpr int RING = 4 * SLOTS * 2 * HALF;
-    static constexpr int O_BYTES = ROWS * (D + 4) * 4;
+    static constexpr int RING = WARPS * SLOTS * 2 * HALF;
+    static constexpr int O_BYTES = WARPS * ROWS * (D + 4) * 4;
     static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;
     static constexpr int Q_BYTES = PARTS * NT * (D / 16) * 256;
-    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + 10 * ROWS * 4 + 4 * SLOTS * 2 * 4;
+    static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + (2 * WARPS + 2) * ROWS * 4 + WARPS * SLOTS * 2 * 4;
     static constexpr int PER_SM = 2 * (SMEM + 1024) <= 227 * 1024 ? 2 : 1;
     static constexpr bool Q_REGS = NT * (D / 16) * PARTS * 2 <= 48;
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128, DecodeShape<T, D, NT>::PER_SM) tree_decode_kernel(const TreeArgs p) {
+__global__ void __launch_bounds__(DecodeShape<T, D, NT>::THREADS, DecodeShape<T, D, NT>::PER_SM) tree_decode_kernel(const TreeArgs p) {
     using S = DecodeShape<T, D, NT>;
-    constexpr int PARTS = S::PARTS, ROWS = S::ROWS, SLOTS = S::SLOTS;
+    constexpr int PARTS = S::PARTS, ROWS = S::ROWS, SLOTS = S::SLOTS, WARPS = S::WARPS;
     constexpr float NEG = -INFINITY;
     extern __shared__ __align__(16) uint8_t smem[];
     uint2 *qfrag = reinterpret_cast<uint2 *>(smem + S::MAIN);
     uint64_t *vis = reinterpret_cast<uint64_t *>(smem + S::MAIN + S::Q_BYTES);
     float *qfac = reinterpret_cast<float *>(vis + ROWS);
-    float *m_w = qfac + ROWS, *l_w = m_w + 4 * ROWS, *m_row = l_w + 4 * ROWS, *l_row = m_row + ROWS;
+    float *m_w = qfac + ROWS, *l_w = m_w + WARPS * ROWS, *m_row = l_w + WARPS * ROWS, *l_row = m_row + ROWS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     int *ids = reinterpret_cast<int *>(l_row + ROWS) + warp * SLOTS * 2;  // [slot][2]: rows of the pool of the group's halves
     const int kvh = blockIdx.y % p.kv_heads, b = blockIdx.z;
@@ -630,13 +643,13 @@ __global__ void __launch_bounds__(128, DecodeShape<T, D, NT>::PER_SM) tree_decod
     {
         int row[SLOTS];
 #pragma unroll
-        for (int j = 0; j < SLOTS - 1; ++j) row[j] = look(g0 + 4 * j);
+        for (int j = 0; j < SLOTS - 1; ++j) row[j] = look(g0 + WARPS * j);
 #pragma unroll
-        for (int j = 0; j < SLOTS - 1; ++j) issue(g0 + 4 * j, j, row[j]);
+        for (int j = 0; j < SLOTS - 1; ++j) issue(g0 + WARPS * j, j, row[j]);
     }
-    int next = look(g0 + 4 * (SLOTS - 1));
+    int next = look(g0 + WARPS * (SLOTS - 1));
 
-    tree_queries<T, D, ROWS, 128>(p, qfrag, vis, qfac, start, row_base, nrows, kvh);
+    tree_queries<T, D, ROWS, WARPS * 32>(p, qfrag, vis, qfac, start, row_base, nrows, kvh);
     __syncthreads();
     uint2 qr[S::Q_REGS ? NT * (D / 16) * PARTS : 1];
     if constexpr (S::Q_REGS) {
@@ -657,11 +670,11 @@ __global__ void __launch_bounds__(128, DecodeShape<T, D, NT>::PER_SM) tree_decod
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = NEG, l[n][0] = l[n][1] = 0.0f;
 
     int slot = 0;
-    for (int grp = g0; grp < g1; grp += 4) {
+    for (int grp = g0; grp < g1; grp += WARPS) {
         asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
         __syncwarp();  // the group is there for every lane, and every lane is done with the slot before
-        issue(grp + 4 * (SLOTS - 1), slot == 0 ? SLOTS - 1 : slot - 1, next);
-        next = look(grp + 4 * SLOTS);
+        issue(grp + WARPS * (SLOTS - 1), slot == 0 ? SLOTS - 1 : slot - 1, next);
+        next = look(grp + WARPS * SLOTS);
         const uint32_t kt = ring + slot * 2 * S::HALF, vt = kt + S::HALF;
         const int key0 = grp * 16;
         const bool drafted = key0 + 16 > ctx;
@@ -819,53 +832,175 @@ __global__ void __launch_bounds__(128, DecodeShape<T, D, NT>::PER_SM) tree_decod
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the ring is done with: O goes over it
-    tree_join<D, NT, 1, 4>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
+    tree_join<D, NT, 1, WARPS>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
 }
 
-// Into how many CTAs (of a cluster) the keys of one set of rows go.  A CTA's time is its keys and, in their measure, about 256
-// for starting, queries and the join; CTAs run in rounds of `slots`.  Sizes the GPU's clusters take; 16 needs asking for.
-inline unsigned tree_split(size_t have, size_t slots, long long keys) {
-    unsigned best = 1;
+// One warp a row: joins the shares' rows, share after share.
+template <int D>
+__global__ void __launch_bounds__(128) tree_gather_kernel(const TreeArgs p, int rows_of_cta, int shares) {
+    constexpr float NEG = -INFINITY;
+    constexpr int V = (D / 4 + 31) / 32;  // float4s of a lane
+    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int kvh = blockIdx.y % p.kv_heads, b = blockIdx.z, row = (int)(blockIdx.y / p.kv_heads) * rows_of_cta + r;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int start = p.node_start[b];
+    int nodes = p.node_start[b + 1] - start;
+    nodes = start < 0 || start > p.tokens ? 0 : min(min(nodes, p.max_nodes), p.tokens - start);
+    if (r >= rows_of_cta || row >= max(nodes, 0) * p.group) return;
+    const size_t pitch = (size_t)rows_of_cta * (D + 4);
+    const float *src = p.part + ((size_t)b * gridDim.y + blockIdx.y) * shares * pitch + (size_t)r * (D + 4);
+    float top = NEG;
+    for (int q = lane; q < shares; q += 32) top = fmaxf(top, src[q * pitch + D]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == NEG ? 0.0f : top;
+    float4 v[V];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int q = 0; q < shares; ++q) {
+        const float k = exp2f(src[q * pitch + D] - ref);
+        sum = fmaf(src[q * pitch + D + 1], k, sum);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (lane + i * 32) * 4;
+            if (c >= D) continue;
+            const float4 x = *reinterpret_cast<const float4 *>(src + q * pitch + c);
+            v[i].x = fmaf(x.x, k, v[i].x), v[i].y = fmaf(x.y, k, v[i].y), v[i].z = fmaf(x.z, k, v[i].z), v[i].w = fmaf(x.w, k, v[i].w);
+        }
+    }
+    float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (lane + i * 32) * 4;
+        if (c >= D) continue;
+        float4 x = v[i];
+        if (sum == 0.0f) {
+            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a row that sees nothing
+        } else {
+            x.x = __fdiv_rn(x.x, sum), x.y = __fdiv_rn(x.y, sum), x.z = __fdiv_rn(x.z, sum), x.w = __fdiv_rn(x.w, sum);
+        }
+        if (p.vec_out) {
+            *reinterpret_cast<float4 *>(dst + c) = x;
+        } else {
+            dst[c] = x.x, dst[c + 1] = x.y, dst[c + 2] = x.z, dst[c + 3] = x.w;
+        }
+    }
+}
+
+// How the keys of one set of rows are split.  A CTA's time is its keys and, in their measure, about 400 for starting,
+// queries and the join.  `resident[i]`: how many clusters of TREE_SIZES[i] CTAs the GPU holds at once (a cluster lies in one
+// GPC: of 148 SMs with one CTA each, 120 serve clusters of 8 and 112 those of 16).  Beyond a cluster's 16 the shares are
+// joined by a second kernel through a workspace, worth about 300 more.
+constexpr int TREE_SIZES[] = {1, 2, 3, 4, 6, 8, 16};
+constexpr int TREE_SIZE_COUNT = 7;
+struct TreeSplit {
+    unsigned shares;
+    bool gather;
+};
+inline TreeSplit tree_split(size_t have, size_t slots, const int *resident, long long keys, bool may_gather) {
+    TreeSplit best = {1, false};
     double least = 1e300;
-    for (unsigned s : {1u, 2u, 3u, 4u, 6u, 8u, 16u}) {
-        if (s > 1 && keys < (long long)s * 2 * TREE_KEYS) break;
-        const double cost = (double)((have * s + slots - 1) / slots) * ((double)keys / s + 256.0);
-        if (cost < least * 0.98) best = s, least = cost;
+    for (int i = 0; i < TREE_SIZE_COUNT; ++i) {
+        const int s = TREE_SIZES[i];
+        if (s > 1 && (keys < (long long)s * 2 * TREE_KEYS || resident[i] < 1)) break;
+        const double cost = (double)((have + resident[i] - 1) / resident[i]) * ((double)keys / s + 400.0);
+        if (cost < least * 0.98) best = {(unsigned)s, false}, least = cost;
+    }
+    const long long most = keys / (2 * TREE_KEYS) < 128 ? keys / (2 * TREE_KEYS) : 128;
+    const long long s = have ? (long long)(slots / have) : 0;  // one full round
+    if (may_gather && s > best.shares) {
+        const long long g = s < most ? s : most;
+        if (g > best.shares && (double)keys / g + 400.0 + 300.0 < least) best = {(unsigned)g, true};
     }
     return best;
 }
 
+// What launching asks of the driver once a kernel and device.
+struct TreeKernelInfo {
+    std::mutex mu;
+    std::atomic<uint64_t> known{0};
+    int resident[64][TREE_SIZE_COUNT];
+};
+
 template <typename K>
-int launch_tree_kernel(nne_ctx *ctx, K kernel, std::atomic<uint64_t> &asked, int threads, size_t smem, int per_sm, int rows_of_cta, const TreeArgs &a,
-                       int sequences, int max_rows, long long max_keys, cudaStream_t s) {
-    const size_t blocks = (size_t)a.kv_heads * ((max_rows + rows_of_cta - 1) / rows_of_cta);
-    if (blocks > 65535 || sequences > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "too many heads or sequences for one launch");
-    NNE_TRY(ensure_dynamic_smem(ctx->device, kernel, smem));
-    const unsigned split = tree_split(blocks * sequences, (size_t)ctx->sm_count * per_sm, max_keys);
-    if (split > 8) {  // clusters of 16 are asked for once a device
-        const uint64_t bit = 1ull << (ctx->device & 63);
-        if (!(asked.load(std::memory_order_acquire) & bit)) {
-            NNE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            asked.fetch_or(bit, std::memory_order_release);
+int tree_kernel_info(const nne_ctx *ctx, K kernel, TreeKernelInfo &info, int threads, size_t smem, const int **resident) {
+    const int dev = ctx->device & 63;
+    if (!(info.known.load(std::memory_order_acquire) >> dev & 1)) {
+        std::lock_guard<std::mutex> lock(info.mu);
+        NNE_TRY(ensure_dynamic_smem(ctx->device, kernel, smem));
+        NNE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (int i = 0; i < TREE_SIZE_COUNT; ++i) {
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)TREE_SIZES[i];
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)TREE_SIZES[i], 64, 1);
+            cfg.blockDim = dim3((unsigned)threads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            info.resident[dev][i] = i == 0 && n < 1 ? 1 : n;
         }
+        info.known.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    *resident = info.resident[dev];
+    return NNE_OK;
+}
+
+template <typename K>
+int launch_tree_kernel(nne_ctx *ctx, K kernel, TreeKernelInfo &info, int threads, size_t smem, int per_sm, int rows_of_cta, int d, const TreeArgs &args,
+                       int sequences, int max_rows, long long max_keys, bool may_gather, cudaStream_t s) {
+    const size_t blocks = (size_t)args.kv_heads * ((max_rows + rows_of_cta - 1) / rows_of_cta);
+    if (blocks > 65535 || sequences > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "too many heads or sequences for one launch");
+    const int *resident;
+    NNE_TRY(tree_kernel_info(ctx, kernel, info, threads, smem, &resident));
+    const TreeSplit split = tree_split(blocks * sequences, (size_t)ctx->sm_count * per_sm, resident, max_keys, may_gather);
+    TreeArgs a = args;
+    void *work = nullptr;
+    if (split.gather) {
+        NNE_CUDA_TRY(cudaMallocAsync(&work, blocks * sequences * split.shares * rows_of_cta * (d + 4) * sizeof(float), s));
+        a.part = static_cast<float *>(work);
     }
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.x = split.gather ? 1 : split.shares;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split, (unsigned)blocks, (unsigned)sequences);
+    cfg.gridDim = dim3(split.shares, (unsigned)blocks, (unsigned)sequences);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     count_launch();
+    if (e == cudaSuccess && split.gather) {
+        cfg.gridDim = dim3((unsigned)((rows_of_cta + 3) / 4), (unsigned)blocks, (unsigned)sequences);
+        cfg.blockDim = dim3(128);
+        cfg.dynamicSmemBytes = 0;
+        cfg.numAttrs = 1;
+        const int shares = (int)split.shares;
+        switch (d) {
+            case 64: e = cudaLaunchKernelEx(&cfg, tree_gather_kernel<64>, a, rows_of_cta, shares); break;
+            case 96: e = cudaLaunchKernelEx(&cfg, tree_gather_kernel<96>, a, rows_of_cta, shares); break;
+            case 128: e = cudaLaunchKernelEx(&cfg, tree_gather_kernel<128>, a, rows_of_cta, shares); break;
+            default: e = cudaLaunchKernelEx(&cfg, tree_gather_kernel<256>, a, rows_of_cta, shares); break;
+        }
+        count_launch();
+    }
+    if (work) cudaFreeAsync(work, s);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(NNE_ERR_CUDA, "tree attention launch failed: %s", cudaGetErrorString(e));
@@ -876,15 +1011,15 @@ int launch_tree_kernel(nne_ctx *ctx, K kernel, std::atomic<uint64_t> &asked, int
 template <typename T, int D, int NT>
 int launch_decode(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
     using S = DecodeShape<T, D, NT>;
-    static std::atomic<uint64_t> asked{0};
-    return launch_tree_kernel(ctx, tree_decode_kernel<T, D, NT>, asked, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, a, sequences, max_rows, max_keys, s);
+    static TreeKernelInfo info;
+    return launch_tree_kernel(ctx, tree_decode_kernel<T, D, NT>, info, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, D, a, sequences, max_rows, max_keys, true, s);
 }
 template <typename T, int D, int NT, int WN, int WK>
 int launch_tree_shape(nne_ctx *ctx, const TreeArgs &a, int sequences, int max_rows, long long max_keys, cudaStream_t s) {
     using S = TreeShape<T, D, NT, WN, WK>;
-    static std::atomic<uint64_t> asked{0};
-    return launch_tree_kernel(ctx, tree_attention_kernel<T, D, NT, WN, WK>, asked, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, a, sequences, max_rows,
-                              max_keys, s);
+    static TreeKernelInfo info;
+    return launch_tree_kernel(ctx, tree_attention_kernel<T, D, NT, WN, WK>, info, S::THREADS, S::SMEM, S::PER_SM, S::ROWS, D, a, sequences, max_rows,
+                              max_keys, false, s);
 }
 
 // Shapes by the rows a key/value head meets at most: the fewest idle MMA columns.  O takes D/16 * NT * 4 registers a
@@ -895,8 +1030,7 @@ int launch_tree_d(nne_ctx *ctx, const TreeArgs &a, int sequences, long long max_
     if (rows <= 8) return launch_decode<T, D, 1>(ctx, a, sequences, rows, max_keys, s);
     if constexpr (D <= 128) {
         if (rows <= 16) return launch_decode<T, D, 2>(ctx, a, sequences, rows, max_keys, s);
-        if (rows <= 32) return launch_tree_shape<T, D, 2, 2, 2>(ctx, a, sequences, rows, max_keys, s);
-        return launch_tree_shape<T, D, 2, 4, 2>(ctx, a, sequences, rows, max_keys, s);
+        return launch_tree_shape<T, D, 2, 2, 2>(ctx, a, sequences, rows, max_keys, s);
     } else {
         if (rows <= 16) return launch_tree_shape<T, D, 1, 2, 2>(ctx, a, sequences, rows, max_keys, s);
         return launch_tree_shape<T, D, 1, 4, 2>(ctx, a, sequences, rows, max_keys, s);
