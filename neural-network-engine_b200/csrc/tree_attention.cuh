@@ -43,6 +43,7 @@ struct TreeArgs {
 
 constexpr int TREE_KEYS = 64;   // keys of a tile
 constexpr int TREE_IDS = 8;     // tiles whose row numbers are held
+constexpr int TREE_SHARES = 128;  // shares that tree_gather_kernel joins at most: one a thread
 
 template <typename T>
 struct TreeType;
@@ -835,34 +836,44 @@ __global__ void __launch_bounds__(DecodeShape<T, D, NT>::THREADS, DecodeShape<T,
     tree_join<D, NT, 1, WARPS>(p, o, m, l, smem, m_w, l_w, m_row, l_row, start, row_base, nrows, kvh);
 }
 
-// One warp a row: joins the shares' rows, share after share.
+// One CTA a row: the weights of its shares (one a thread; at most 128), then each warp every fourth share, then the warps in
+// order.  (One warp a row, share after share, took longer than the attention: 19 us for 37 shares.)
 template <int D>
-__global__ void __launch_bounds__(128) tree_gather_kernel(const TreeArgs p, int rows_of_cta, int shares) {
-    constexpr float NEG = -INFINITY;
+__global__ void __launch_bounds__(TREE_SHARES) tree_gather_kernel(const TreeArgs p, int rows_of_cta, int shares) {
     constexpr int V = (D / 4 + 31) / 32;  // float4s of a lane
-    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5);
+    __shared__ float weight[TREE_SHARES], tops[4], sums[4];
+    __shared__ __align__(16) float acc[4][D];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x;
     const int kvh = blockIdx.y % p.kv_heads, b = blockIdx.z, row = (int)(blockIdx.y / p.kv_heads) * rows_of_cta + r;
     grid_dependency_wait();
     grid_launch_dependents();
     const int start = p.node_start[b];
     int nodes = p.node_start[b + 1] - start;
     nodes = start < 0 || start > p.tokens ? 0 : min(min(nodes, p.max_nodes), p.tokens - start);
-    if (r >= rows_of_cta || row >= max(nodes, 0) * p.group) return;
+    if (row >= max(nodes, 0) * p.group) return;
     const size_t pitch = (size_t)rows_of_cta * (D + 4);
     const float *src = p.part + ((size_t)b * gridDim.y + blockIdx.y) * shares * pitch + (size_t)r * (D + 4);
-    float top = NEG;
-    for (int q = lane; q < shares; q += 32) top = fmaxf(top, src[q * pitch + D]);
+    const float m = tid < shares ? src[tid * pitch + D] : -INFINITY, l = tid < shares ? src[tid * pitch + D + 1] : 0.0f;
+    float top = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float ref = top == NEG ? 0.0f : top;
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float w = exp2f(m - (top == -INFINITY ? 0.0f : top));
+    weight[tid] = w;
+    float sum = l * w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    sum = sums[0] + sums[1] + sums[2] + sums[3];
     float4 v[V];
-    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-    for (int q = 0; q < shares; ++q) {
-        const float k = exp2f(src[q * pitch + D] - ref);
-        sum = fmaf(src[q * pitch + D + 1], k, sum);
+    for (int q = warp; q < shares; q += 4) {
+        const float k = weight[q];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = (lane + i * 32) * 4;
@@ -871,23 +882,13 @@ __global__ void __launch_bounds__(128) tree_gather_kernel(const TreeArgs p, int 
             v[i].x = fmaf(x.x, k, v[i].x), v[i].y = fmaf(x.y, k, v[i].y), v[i].z = fmaf(x.z, k, v[i].z), v[i].w = fmaf(x.w, k, v[i].w);
         }
     }
-    float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = (lane + i * 32) * 4;
-        if (c >= D) continue;
-        float4 x = v[i];
-        if (sum == 0.0f) {
-            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a row that sees nothing
-        } else {
-            x.x = __fdiv_rn(x.x, sum), x.y = __fdiv_rn(x.y, sum), x.z = __fdiv_rn(x.z, sum), x.w = __fdiv_rn(x.w, sum);
-        }
-        if (p.vec_out) {
-            *reinterpret_cast<float4 *>(dst + c) = x;
-        } else {
-            dst[c] = x.x, dst[c + 1] = x.y, dst[c + 2] = x.z, dst[c + 3] = x.w;
-        }
-    }
+    for (int i = 0; i < V; ++i)
+        if ((lane + i * 32) * 4 < D) *reinterpret_cast<float4 *>(&acc[warp][(lane + i * 32) * 4]) = v[i];
+    __syncthreads();
+    float *dst = p.out + (size_t)(start + row / p.group) * p.out_stride + (size_t)(kvh * p.group + row % p.group) * D;
+    for (int c = tid; c < D; c += TREE_SHARES)
+        dst[c] = sum == 0.0f ? 0.0f : __fdiv_rn(acc[0][c] + acc[1][c] + acc[2][c] + acc[3][c], sum);  // 0: a row that sees nothing
 }
 
 // How the keys of one set of rows are split.  A CTA's time is its keys and, in their measure, about 400 for starting,
@@ -909,7 +910,7 @@ inline TreeSplit tree_split(size_t have, size_t slots, const int *resident, long
         const double cost = (double)((have + resident[i] - 1) / resident[i]) * ((double)keys / s + 400.0);
         if (cost < least * 0.98) best = {(unsigned)s, false}, least = cost;
     }
-    const long long most = keys / (2 * TREE_KEYS) < 128 ? keys / (2 * TREE_KEYS) : 128;
+    const long long most = keys / (2 * TREE_KEYS) < TREE_SHARES ? keys / (2 * TREE_KEYS) : TREE_SHARES;
     const long long s = have ? (long long)(slots / have) : 0;  // one full round
     if (may_gather && s > best.shares) {
         const long long g = s < most ? s : most;
@@ -987,8 +988,8 @@ int launch_tree_kernel(nne_ctx *ctx, K kernel, TreeKernelInfo &info, int threads
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     count_launch();
     if (e == cudaSuccess && split.gather) {
-        cfg.gridDim = dim3((unsigned)((rows_of_cta + 3) / 4), (unsigned)blocks, (unsigned)sequences);
-        cfg.blockDim = dim3(128);
+        cfg.gridDim = dim3((unsigned)rows_of_cta, (unsigned)blocks, (unsigned)sequences);
+        cfg.blockDim = dim3(TREE_SHARES);
         cfg.dynamicSmemBytes = 0;
         cfg.numAttrs = 1;
         const int shares = (int)split.shares;
