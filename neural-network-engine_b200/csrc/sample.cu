@@ -11,11 +11,14 @@
 // other's shared memory: the row's later passes come from L1, and nothing of it goes through global memory or a
 // second launch.
 //
-// Nothing is sorted.  A logit's bits, made monotone, are its key; top-k and top-p are each a search for the key at which a
-// count or a mass reaches its target, 256 buckets a pass, first by distance from the maximum in units of T / 8 and
-// then by the key's bits, until a bucket is one key; equal keys are cut off by index.  Masses are integers in units
-// of 2^-40 of the largest weight, 64 bits wide: sums of them do not depend on order, so atomics leave results the same from run to run,
-// and every pass sees the same totals.
+// Three passes where the settings leave few tokens, as they nearly always do: the maximum; counts and masses by distance from
+// it, in 256 buckets of T / 16, which show up to which bucket the settings can reach; and the tokens up to that bucket, at most 1024,
+// into a list in the first CTA's shared memory.  That CTA sorts them, cuts the list and draws.
+// Where more are left, nothing is sorted: a logit's bits, made monotone, are its key; top-k and top-p are each a
+// search for the key at which a count or a mass reaches its target, 256 buckets a pass, first by distance from the maximum and
+// then by the key's bits, until a bucket is one key; equal keys are cut off by index.
+// Masses are integers in units of 2^-40 of the largest weight, 64 bits wide: sums of them do not depend on order, so atomics
+// leave results the same from run to run, and every pass sees the same totals.
 #include <math.h>
 
 #include "common.cuh"
@@ -26,6 +29,8 @@ namespace {
 
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32;
 constexpr int SM_BUCKETS = 256;
+constexpr float SM_PER_T = 16.0f;  // buckets of a temperature's width
+constexpr int SM_LIST = 1024;      // tokens of the list: two a thread
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf (and of NaN, which counts as -inf)
 
 struct SampleArgs {
@@ -53,6 +58,11 @@ struct Shared {
     unsigned found;
     int bucket;
     unsigned long long above;
+    unsigned count[SM_BUCKETS], all_count[SM_BUCKETS];
+    unsigned long long list[SM_LIST];
+    unsigned long long rest[2];
+    unsigned listed;
+    unsigned kept;
 };
 
 __device__ __forceinline__ void cluster_meet() {
@@ -71,6 +81,19 @@ __device__ __forceinline__ unsigned ld_cluster_u32(const void *p, unsigned rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer) : "memory");
     return v;
+}
+
+__device__ __forceinline__ unsigned add_cluster_u32(const void *p, unsigned rank, unsigned v) {
+    uint32_t peer;
+    unsigned old;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(peer), "r"(v) : "memory");
+    return old;
+}
+__device__ __forceinline__ void st_cluster_u64(const void *p, unsigned rank, unsigned long long v) {
+    uint32_t peer;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer), "l"(v) : "memory");
 }
 
 struct Row {
@@ -274,6 +297,248 @@ struct Row {
     }
 };
 
+// A block's prefix sums of two values a thread (places 2t and 2t + 1): `v` becomes the sums up to and with each.
+__device__ __forceinline__ void block_prefix(Shared *s, unsigned long long (&v)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned long long own = v[0] + v[1];
+    unsigned long long up = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += u;
+    }
+    __syncthreads();
+    if (lane == 31) s->warp[warp] = up;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) up += s->warp[w];
+    v[1] = up;
+    v[0] = up - own + v[0];
+}
+
+// Sorts the first `n` (a power of two) of the list, largest first; all threads.
+__device__ __forceinline__ void sort_list(unsigned long long *x, unsigned n) {
+    for (unsigned size = 2; size <= n; size <<= 1)
+        for (unsigned gap = size >> 1; gap > 0; gap >>= 1) {
+            __syncthreads();
+            for (unsigned i = threadIdx.x; i < n / 2; i += SM_THREADS) {
+                const unsigned lo = ((i & ~(gap - 1)) << 1) | (i & (gap - 1)), hi = lo | gap;
+                const unsigned long long a = x[lo], b = x[hi];
+                if ((a < b) == ((lo & size) == 0)) x[lo] = b, x[hi] = a;
+            }
+        }
+    __syncthreads();
+}
+
+struct Settings {
+    int k;          // 0: off
+    float top_p;    // >= 1: off
+    float min_p;    // <= 0: off; at most 1
+    float u;
+};
+
+// The token, where the settings leave at most SM_LIST, or -2.  All CTAs return the same.
+__device__ __noinline__ int draw_from_list(Row &r, Settings set) {
+    Shared *s = r.s;
+    const float inv = __fdiv_rn(SM_PER_T, r.temperature);
+    const bool by_mass = set.top_p < 1.0f;
+    auto bucket_of = [&](float x) {  // never falls as x falls; SM_BUCKETS: farther off than the buckets reach
+        const float d = x == r.top ? 0.0f : (r.top - x) * inv;
+        return d < (float)SM_BUCKETS ? (int)d : SM_BUCKETS;
+    };
+    unsigned rest = 0;
+    unsigned long long rest_mass = 0;
+    r.each([&](unsigned, float x) {
+        if (key_of(x) <= KEY_NONE) return;
+        const int j = bucket_of(x);
+        if (j < SM_BUCKETS) {
+            atomicAdd(&s->count[j], 1u);
+            if (by_mass) atomicAdd(&s->mass[0][j], Row::units(r.weight(x)));
+        } else {
+            ++rest;
+            if (by_mass && set.k == 0) rest_mass += Row::units(r.weight(x));  // with top-k only the list's masses matter
+        }
+    });
+    const unsigned long long mine = r.block_sum(rest), mine_mass = r.block_sum(rest_mass);
+    if (threadIdx.x == 0) s->rest[0] = mine, s->rest[1] = mine_mass;
+    cluster_meet();
+    unsigned long long others = 0, others_mass = 0;
+    for (unsigned q = 0; q < r.ranks; ++q) {
+        others += ld_cluster_u64(&s->rest[0], q);
+        others_mass += ld_cluster_u64(&s->rest[1], q);
+    }
+    if (threadIdx.x < SM_BUCKETS) {
+        unsigned c = 0;
+        unsigned long long m = 0;
+        for (unsigned q = 0; q < r.ranks; ++q) {
+            c += ld_cluster_u32(&s->count[threadIdx.x], q);
+            if (by_mass) m += ld_cluster_u64(&s->mass[0][threadIdx.x], q);
+        }
+        s->all_count[threadIdx.x] = c;
+        s->all[threadIdx.x] = m;
+    }
+    __syncthreads();
+    // Sums up to and with each bucket; thread t has buckets 2t and 2t + 1.
+    unsigned long long counts[2] = {0, 0}, masses[2] = {0, 0};
+    if (threadIdx.x < SM_BUCKETS / 2) {
+        counts[0] = s->all_count[2 * threadIdx.x], counts[1] = s->all_count[2 * threadIdx.x + 1];
+        masses[0] = s->all[2 * threadIdx.x], masses[1] = s->all[2 * threadIdx.x + 1];
+    }
+    block_prefix(s, counts);
+    if (by_mass) block_prefix(s, masses);
+    __syncthreads();
+    if (threadIdx.x < SM_BUCKETS / 2) {
+        s->all_count[2 * threadIdx.x] = (unsigned)counts[0], s->all_count[2 * threadIdx.x + 1] = (unsigned)counts[1];
+        s->all[2 * threadIdx.x] = masses[0], s->all[2 * threadIdx.x + 1] = masses[1];
+    }
+    __syncthreads();
+    const unsigned long long tokens = s->all_count[SM_BUCKETS - 1] + others;
+    const unsigned long long mass = s->all[SM_BUCKETS - 1] + others_mass;
+    if (set.k > 0 && (unsigned long long)set.k >= tokens) {
+        if (by_mass && others) return -2;  // the mass beyond the buckets was not summed
+        set.k = 0;
+    }
+    // The last bucket that each setting can reach into.
+    auto first = [&](auto &&reached) {  // of the buckets; SM_BUCKETS: none
+        int lo = 0, hi = SM_BUCKETS;
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (reached(mid)) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    };
+    int last = SM_BUCKETS;
+    if (set.k > 0) last = first([&](int j) { return s->all_count[j] >= (unsigned)set.k; });
+    if (by_mass && set.k == 0) {
+        const double want = (double)set.top_p * (double)mass;
+        const int j = first([&](int q) { return (double)s->all[q] >= want; });
+        last = j < last ? j : last;
+    }
+    if (set.min_p > 0.0f && !(by_mass && set.k > 0)) {  // top-p of a top-k needs the mass of all of these
+        const float far = -logf(set.min_p) * SM_PER_T;
+        if (far < (float)(SM_BUCKETS - 2) && (int)far + 1 < last) last = (int)far + 1;
+    }
+    const unsigned n = last < SM_BUCKETS ? s->all_count[last] : SM_LIST + 1;
+    if (n > SM_LIST) return -2;
+
+    r.each([&](unsigned i, float x) {
+        const uint32_t key = key_of(x);
+        const bool in = key > KEY_NONE && bucket_of(x) <= last;
+        if (in) st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key << 32 | (0xffffffffu - i));
+    });
+    cluster_meet();
+    if (r.rank != 0) return 0;
+
+    unsigned size = 2;
+    while (size < n) size <<= 1;
+    for (unsigned i = n + threadIdx.x; i < size; i += SM_THREADS) s->list[i] = 0;
+    sort_list(s->list, size);
+    const unsigned at = 2 * threadIdx.x;
+    unsigned long long entry[2], w[2], upto[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        entry[e] = at + e < n ? s->list[at + e] : 0;
+        const float x = logit_of((uint32_t)(entry[e] >> 32));
+        w[e] = at + e < n ? Row::units(r.weight(x)) : 0;
+        upto[e] = w[e];
+    }
+    block_prefix(s, upto);
+    const unsigned most = set.k > 0 ? (unsigned)set.k : SM_LIST;  // top-k: places below this (n >= k)
+    __syncthreads();
+    if (threadIdx.x == 0) s->kept = 0;
+    if (set.k > 0 && at <= most - 1 && most - 1 < at + 2) s->above = upto[(most - 1) & 1];
+    __syncthreads();
+    const unsigned long long of = set.k > 0 ? s->above : mass;
+    const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)of) : 1ull;
+    unsigned keeps = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const unsigned place = at + e;
+        bool in = place < n && place < most;
+        if (by_mass) in = in && (place == 0 || upto[e] - w[e] < target);
+        if (set.min_p > 0.0f) in = in && r.weight(logit_of((uint32_t)(entry[e] >> 32))) >= set.min_p;
+        keeps += in;
+    }
+    atomicAdd(&s->kept, keeps);
+    __syncthreads();
+    const unsigned kept = s->kept;  // the first places: each condition holds up to some place
+    // In index order: sorted by index, falling, from the back.
+    unsigned ksize = 2;
+    while (ksize < kept) ksize <<= 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (at + e < ksize) s->list[at + e] = at + e < kept ? (entry[e] << 32) | (entry[e] >> 32) : 0;  // (2^32 - 1 - index, key): low indices first
+    sort_list(s->list, ksize);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        entry[e] = at + e < kept ? s->list[at + e] : 0;
+        upto[e] = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
+    }
+    block_prefix(s, upto);
+    if (threadIdx.x == SM_THREADS - 1) s->above = upto[1];
+    __syncthreads();
+    const unsigned long long sum = s->above;
+    const double point = (double)set.u * (double)sum;
+    const unsigned long long want = point < (double)sum ? min((unsigned long long)point, sum - 1) : sum - 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const unsigned long long mass_here = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
+        if (mass_here && upto[e] > want && upto[e] - mass_here <= want) s->found = 0xffffffffu - (unsigned)(entry[e] >> 32);
+    }
+    __syncthreads();
+    return (int)s->found;
+}
+
+// The token, whatever the settings leave.
+__device__ __noinline__ int draw_by_search(Row &r, uint32_t top_key, unsigned vocab, Settings set) {
+    uint32_t cut = KEY_NONE + 1;  // kept: key > cut, or key == cut and index <= cut_index
+    unsigned cut_index = 0xffffffffu;
+    auto kept = [&](unsigned i, float x) {
+        const uint32_t key = key_of(x);
+        return key > cut || (key == cut && i <= cut_index);
+    };
+    if (set.k > 0) {
+        const unsigned long long k = (unsigned long long)set.k;
+        auto one = [&](unsigned, float x) { return (unsigned long long)(key_of(x) > KEY_NONE); };
+        if (r.total(one) > k) {
+            unsigned long long above, at;
+            const uint32_t key = r.search(one, top_key, k, &above, &at);
+            if (above + at > k)
+                cut_index = r.locate([&](unsigned, float x) { return (unsigned long long)(key_of(x) == key); },
+                                     [&](unsigned long long) { return k - above - 1; });
+            cut = key;
+        }
+    }
+    if (set.top_p < 1.0f) {
+        auto mass = [&](unsigned i, float x) { return kept(i, x) ? Row::units(r.weight(x)) : 0ull; };
+        const unsigned long long sum = r.total(mass);
+        unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)sum) : 1ull;
+        target = target < 1 ? 1 : (target > sum ? sum : target);
+        unsigned long long above, at;
+        const uint32_t key = r.search(mass, top_key, target, &above, &at);
+        const unsigned long long each = Row::units(r.weight(logit_of(key)));
+        const unsigned long long have = at / each, need = (target - above + each - 1) / each;
+        if (need < have) {
+            const unsigned index = r.locate([&](unsigned i, float x) { return (unsigned long long)(key_of(x) == key && kept(i, x)); },
+                                            [&](unsigned long long) { return need - 1; });
+            cut_index = index;
+        } else if (key != cut) {
+            cut_index = 0xffffffffu;
+        }
+        cut = key;
+    }
+    return (int)r.locate(
+        [&](unsigned i, float x) {
+            if (!kept(i, x)) return 0ull;
+            const float w = r.weight(x);
+            return w < set.min_p ? 0ull : Row::units(w);
+        },
+        [&](unsigned long long sum) {
+            const double at = (double)set.u * (double)sum;
+            return at < (double)sum ? min((unsigned long long)at, sum - 1) : sum - 1;
+        });
+}
+
 __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) {
     __shared__ Shared sh;
     grid_dependency_wait();
@@ -291,6 +556,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     r.begin = min(cta_begin + (threadIdx.x >> 5) * warp_span, cta_end);
     r.end = min(r.begin + warp_span, cta_end);
     for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
+    if (threadIdx.x < SM_BUCKETS) sh.count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.listed = 0;
 
     // The largest logit and where it is first.
     unsigned long long best = 0;
@@ -313,57 +580,22 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     } else {
         r.top = logit_of(top_key);
         r.temperature = t;
-        uint32_t cut = KEY_NONE + 1;  // kept: key > cut, or key == cut and index <= cut_index
-        unsigned cut_index = 0xffffffffu;
-        auto kept = [&](unsigned i, float x) {
-            const uint32_t key = key_of(x);
-            return key > cut || (key == cut && i <= cut_index);
-        };
-        const int k = p.top_k ? p.top_k[row] : 0;
-        if (k > 0 && (unsigned)k < p.vocab) {
-            auto one = [&](unsigned, float x) { return (unsigned long long)(key_of(x) > KEY_NONE); };
-            if (r.total(one) > (unsigned long long)k) {
-                unsigned long long above, at;
-                const uint32_t key = r.search(one, top_key, (unsigned long long)k, &above, &at);
-                if (above + at > (unsigned long long)k)
-                    cut_index = r.locate([&](unsigned, float x) { return (unsigned long long)(key_of(x) == key); },
-                                         [&](unsigned long long) { return (unsigned long long)k - above - 1; });
-                cut = key;
-            }
+        Settings set;
+        set.k = p.top_k ? p.top_k[row] : 0;
+        set.k = set.k > 0 && (unsigned)set.k < p.vocab ? set.k : 0;
+        set.top_p = p.top_p ? p.top_p[row] : 1.0f;
+        set.top_p = set.top_p < 1.0f ? set.top_p : 1.0f;  // NaN: off
+        set.min_p = p.min_p ? p.min_p[row] : 0.0f;
+        set.min_p = set.min_p > 0.0f ? fminf(set.min_p, 1.0f) : 0.0f;
+        const float u = p.uniform[row];
+        set.u = u > 0.0f ? u : 0.0f;
+        token = -2;
+        if (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f) token = draw_from_list(r, set);
+        if (token == -2) {
+            cluster_meet();  // the buckets have been read by everybody
+            for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
+            token = draw_by_search(r, top_key, p.vocab, set);
         }
-        const float top_p = p.top_p ? p.top_p[row] : 1.0f;
-        if (top_p < 1.0f) {
-            auto mass = [&](unsigned i, float x) { return kept(i, x) ? Row::units(r.weight(x)) : 0ull; };
-            const unsigned long long sum = r.total(mass);
-            unsigned long long target = top_p > 0.0f ? (unsigned long long)ceil((double)top_p * (double)sum) : 1ull;
-            target = target < 1 ? 1 : (target > sum ? sum : target);
-            unsigned long long above, at;
-            const uint32_t key = r.search(mass, top_key, target, &above, &at);
-            const unsigned long long each = Row::units(r.weight(logit_of(key)));
-            const unsigned long long have = at / each, need = (target - above + each - 1) / each;
-            if (need < have) {
-                const unsigned index = r.locate([&](unsigned i, float x) { return (unsigned long long)(key_of(x) == key && kept(i, x)); },
-                                                [&](unsigned long long) { return need - 1; });
-                cut_index = index;
-            } else if (key != cut) {
-                cut_index = 0xffffffffu;
-            }
-            cut = key;
-        }
-        float min_p = p.min_p ? p.min_p[row] : 0.0f;
-        min_p = min_p > 1.0f ? 1.0f : min_p;
-        float u = p.uniform[row];
-        u = u > 0.0f ? u : 0.0f;
-        token = (int)r.locate(
-            [&](unsigned i, float x) {
-                if (!kept(i, x)) return 0ull;
-                const float w = r.weight(x);
-                return w < min_p ? 0ull : Row::units(w);
-            },
-            [&](unsigned long long sum) {
-                const double at = (double)u * (double)sum;
-                return at < (double)sum ? min((unsigned long long)at, sum - 1) : sum - 1;
-            });
     }
     if (r.rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
     cluster_meet();  // nobody leaves while a peer may still read its shared memory

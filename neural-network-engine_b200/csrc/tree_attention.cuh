@@ -566,13 +566,14 @@ struct DecodeShape {
     static constexpr int ROWS = 8 * NT, THREADS = WARPS * 32;
     static constexpr int PITCH = 2 * D + 16;
     static constexpr int HALF = 16 * PITCH;                 // 16 keys; a slot is keys and values
-    static constexpr int SLOTS = D <= 64 ? 5 : 3;
+    static constexpr int SLOTS = 3;
     static constexpr int RING = WARPS * SLOTS * 2 * HALF;
     static constexpr int O_BYTES = WARPS * ROWS * (D + 4) * 4;
     static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;
     static constexpr int Q_BYTES = PARTS * NT * (D / 16) * 256;
     static constexpr int SMEM = MAIN + Q_BYTES + ROWS * 8 + ROWS * 4 + (2 * WARPS + 2) * ROWS * 4 + WARPS * SLOTS * 2 * 4;
-    static constexpr int PER_SM = 2 * (SMEM + 1024) <= 227 * 1024 ? 2 : 1;
+    static constexpr int FIT = 227 * 1024 / (SMEM + 1024);
+    static constexpr int PER_SM = FIT < 1 ? 1 : (FIT > 3 ? 3 : FIT);  // three: 168 registers a thread
     static constexpr bool Q_REGS = NT * (D / 16) * PARTS * 2 <= 48;
 };
 
