@@ -14,7 +14,8 @@
 // Three passes where the settings leave few tokens, as they nearly always do: the maximum; counts and masses by distance from
 // it, in 256 buckets of T / 16, which show up to which bucket the settings can reach; and the tokens up to that bucket, at most 1024,
 // into a list in the first CTA's shared memory.  That CTA sorts them, cuts the list and draws.
-// Where more are left, nothing is sorted: a logit's bits, made monotone, are its key; top-k and top-p are each a
+// Where more are left and one setting cuts them, the list holds the bucket of the cut, and two passes draw from what is above it.
+// Else nothing is sorted: a logit's bits, made monotone, are its key; top-k and top-p are each a
 // search for the key at which a count or a mass reaches its target, 256 buckets a pass, first by distance from the maximum and
 // then by the key's bits, until a bucket is one key; equal keys are cut off by index.
 // Masses are integers in units of 2^-40 of the largest weight, 64 bits wide: sums of them do not depend on order, so atomics
@@ -102,11 +103,14 @@ struct Row {
     unsigned begin, end;     // this warp's indices
     unsigned rank, ranks;
     int meeting, round;      // which of the alternating words and bucket sets is next
-    float top, temperature;
+    float top, temperature, scale;
 
-    // A token's mass in units of 2^-40 of the largest.
-    __device__ __forceinline__ float weight(float x) const { return x == top ? 1.0f : expf(__fdiv_rn(x - top, temperature)); }
-    __device__ __forceinline__ static unsigned long long units(float w) { return __float2ull_rn(w * 0x1p40f); }
+    // A token's weight, and that in units of 2^-40 (the rest of a unit is dropped).  scale: log2(e) / T.
+    __device__ __forceinline__ float weight(float x) const { return x == top ? 1.0f : exp2f(fmaxf(x - top, -3.402823466e38f) * scale); }
+    __device__ __forceinline__ static unsigned long long units(float w) {
+        const uint32_t b = __float_as_uint(w);  // 0 <= w <= 1: 24 bits of mantissa, an exponent of at most 127
+        return ((unsigned long long)((b & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (b >> 23), 63u);
+    }
 
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
@@ -207,6 +211,21 @@ struct Row {
         }
         cluster_meet();
         return ld_cluster_u32(&s->found, owner);
+    }
+
+    // The draw itself: the first index at which the mass of what `kept` and min_p leave exceeds u * that mass.
+    template <typename F>
+    __device__ __forceinline__ unsigned draw(F &&kept, float min_p, float u) {
+        return locate(
+            [&](unsigned i, float x) {
+                if (!kept(i, x)) return 0ull;
+                const float w = weight(x);
+                return w < min_p ? 0ull : units(w);
+            },
+            [&](unsigned long long sum) {
+                const double at = (double)u * (double)sum;
+                return at < (double)sum ? min((unsigned long long)at, sum - 1) : sum - 1;
+            });
     }
 
     // The largest key t with sum of f over keys >= t reaching `target` (>= 1), where the sum over all keys in
@@ -418,15 +437,49 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
         const float far = -logf(set.min_p) * SM_PER_T;
         if (far < (float)(SM_BUCKETS - 2) && (int)far + 1 < last) last = (int)far + 1;
     }
-    const unsigned n = last < SM_BUCKETS ? s->all_count[last] : SM_LIST + 1;
-    if (n > SM_LIST) return -2;
+    if (last == SM_BUCKETS) return -2;
+    // More than the list holds up to there: then the last bucket alone, to find where the one setting that cuts ends in it.
+    const bool cut_only = s->all_count[last] > SM_LIST;
+    const unsigned from = cut_only && last > 0 ? s->all_count[last - 1] : 0;
+    const unsigned n = s->all_count[last] - from;
+    if (n > SM_LIST || (cut_only && by_mass && set.k > 0)) return -2;
+    const unsigned long long mass_from = cut_only && last > 0 ? s->all[last - 1] : 0;
 
     r.each([&](unsigned i, float x) {
         const uint32_t key = key_of(x);
-        const bool in = key > KEY_NONE && bucket_of(x) <= last;
-        if (in) st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key << 32 | (0xffffffffu - i));
+        const int j = bucket_of(x);
+        if (key > KEY_NONE && j <= last && (!cut_only || j == last))
+            st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key << 32 | (0xffffffffu - i));
     });
     cluster_meet();
+    if (cut_only) {
+        // min_p needs no cut of its own: the draw looks at the weights
+        if (r.rank == 0) {
+            unsigned size = 2;
+            while (size < n) size <<= 1;
+            for (unsigned i = n + threadIdx.x; i < size; i += SM_THREADS) s->list[i] = 0;
+            sort_list(s->list, size);
+            const unsigned at = 2 * threadIdx.x;
+            unsigned long long w[2], upto[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                upto[e] = w[e] = at + e < n && by_mass ? Row::units(r.weight(logit_of((uint32_t)(s->list[at + e] >> 32)))) : 0;
+            // nothing cuts in the bucket: min_p ended the buckets there
+            if (threadIdx.x == 0) s->above = n ? s->list[n - 1] : (unsigned long long)(KEY_NONE + 1) << 32;
+            block_prefix(s, upto);
+            const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)mass) : 1ull;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool cuts = set.k > 0 ? from + at + e + 1 == (unsigned)set.k
+                                            : by_mass && w[e] && mass_from + upto[e] - w[e] < target && mass_from + upto[e] >= target;
+                if (at + e < n && cuts) s->above = s->list[at + e];
+            }
+        }
+        cluster_meet();
+        const unsigned long long cut = ld_cluster_u64(&s->above, 0);
+        cluster_meet();  // rank 0 goes on to use the word
+        return (int)r.draw([&](unsigned i, float x) { return ((unsigned long long)key_of(x) << 32 | (0xffffffffu - i)) >= cut; }, set.min_p, set.u);
+    }
     if (r.rank != 0) return 0;
 
     unsigned size = 2;
@@ -527,16 +580,7 @@ __device__ __noinline__ int draw_by_search(Row &r, uint32_t top_key, unsigned vo
         }
         cut = key;
     }
-    return (int)r.locate(
-        [&](unsigned i, float x) {
-            if (!kept(i, x)) return 0ull;
-            const float w = r.weight(x);
-            return w < set.min_p ? 0ull : Row::units(w);
-        },
-        [&](unsigned long long sum) {
-            const double at = (double)set.u * (double)sum;
-            return at < (double)sum ? min((unsigned long long)at, sum - 1) : sum - 1;
-        });
+    return (int)r.draw(kept, set.min_p, set.u);
 }
 
 __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) {
@@ -559,27 +603,23 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     if (threadIdx.x < SM_BUCKETS) sh.count[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.listed = 0;
 
-    // The largest logit and where it is first.
-    unsigned long long best = 0;
-    r.each([&](unsigned i, float x) {
-        const unsigned long long v = (unsigned long long)key_of(x) << 32 | (0xffffffffu - i);
-        best = v > best ? v : best;
-    });
-    const void *w = r.tell(r.block_max(best));
-    for (unsigned q = 0; q < r.ranks; ++q) {
-        const unsigned long long v = ld_cluster_u64(w, q);
-        best = v > best || q == 0 ? v : best;
-    }
-    const uint32_t top_key = (uint32_t)(best >> 32);
+    // The largest logit (NaN is passed over).
+    float top = -INFINITY;
+    r.each([&](unsigned, float x) { top = fmaxf(top, x); });
+    uint32_t top_key = 0;
+    const void *w = r.tell(r.block_max(key_of(top)));
+    for (unsigned q = 0; q < r.ranks; ++q) top_key = max(top_key, (uint32_t)ld_cluster_u64(w, q));
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     int token;
     if (top_key <= KEY_NONE) {
         token = -1;  // no logit to choose
     } else if (!(t > 0.0f)) {
-        token = (int)(0xffffffffu - (uint32_t)best);
+        token = (int)r.locate([&](unsigned, float x) { return (unsigned long long)(key_of(x) == top_key); }, [](unsigned long long) { return 0ull; });
     } else {
         r.top = logit_of(top_key);
         r.temperature = t;
+        // finite, so that 0 * scale is 0; beside an infinite logit all others weigh nothing, whatever the temperature
+        r.scale = isinf(r.top) ? 3.402823466e38f : fminf(__fdiv_rn(1.44269504088896340736f, t), 3.402823466e38f);
         Settings set;
         set.k = p.top_k ? p.top_k[row] : 0;
         set.k = set.k > 0 && (unsigned)set.k < p.vocab ? set.k : 0;
@@ -620,6 +660,8 @@ extern "C" int nne_sample_dev(nne_ctx *ctx, const nne_sample *a, void *stream) {
     // CTAs a row: as many as leave each at least 2048 logits (four a thread), up to the 8 of a portable cluster.
     unsigned ranks = 1;
     while (ranks < 8 && a->vocab >= (size_t)ranks * 2 * 2048) ranks *= 2;
+    // and not more than run at once, two an SM: a second round would wait for the first one's meetings
+    while (ranks > 1 && a->rows * ranks > 2 * (size_t)ctx->sm_count) ranks /= 2;
     SampleArgs p = {a->logits, a->row_stride, (unsigned)a->vocab, a->temperature, a->top_p, a->min_p, a->uniform, a->top_k, a->tokens};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
