@@ -12,9 +12,10 @@
 // second launch.
 //
 // Three passes where the settings leave few tokens, as they nearly always do: the maximum; counts and masses by distance from
-// it, in 256 buckets of T / 16, which show up to which bucket the settings can reach; and the tokens up to that bucket, at most 1024,
+// it, in 256 buckets of T / 16 and T / 4, which show up to which bucket the settings can reach; and the tokens up to that bucket, at most 1024,
 // into a list in the first CTA's shared memory.  That CTA sorts them, cuts the list and draws.
-// Where more are left and one setting cuts them, the list holds the bucket of the cut, and two passes draw from what is above it.
+// Where more are left and one setting cuts them, the list holds the bucket of the cut (or, a pass more, a 256th of it), and two passes
+// draw from what is above it.
 // Else nothing is sorted: a logit's bits, made monotone, are its key; top-k and top-p are each a
 // search for the key at which a count or a mass reaches its target, 256 buckets a pass, first by distance from the maximum and
 // then by the key's bits, until a bucket is one key; equal keys are cut off by index.
@@ -31,6 +32,7 @@ namespace {
 constexpr int SM_THREADS = 512, SM_WARPS = SM_THREADS / 32;
 constexpr int SM_BUCKETS = 256;
 constexpr float SM_PER_T = 16.0f;  // buckets of a temperature's width
+constexpr int SM_FINE = 192;       // of them, that many; the others are four times as wide
 constexpr int SM_LIST = 1024;      // tokens of the list: two a thread
 constexpr uint32_t KEY_NONE = 0x007fffffu;  // the key of -inf (and of NaN, which counts as -inf)
 
@@ -59,9 +61,8 @@ struct Shared {
     unsigned found;
     int bucket;
     unsigned long long above;
-    unsigned count[SM_BUCKETS], all_count[SM_BUCKETS];
+    unsigned count[2][SM_BUCKETS], low[2][SM_BUCKETS], high[2][SM_BUCKETS], all_count[SM_BUCKETS];
     unsigned long long list[SM_LIST];
-    unsigned long long rest[2];
     unsigned listed;
     unsigned kept;
 };
@@ -97,32 +98,73 @@ __device__ __forceinline__ void st_cluster_u64(const void *p, unsigned rank, uns
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer), "l"(v) : "memory");
 }
 
+// A block's prefix sums of two values a thread (places 2t and 2t + 1): `v` becomes the sums up to and with each.
+__device__ __forceinline__ void block_prefix(Shared *s, unsigned long long (&v)[2]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned long long own = v[0] + v[1];
+    unsigned long long up = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += u;
+    }
+    __syncthreads();
+    if (lane == 31) s->warp[warp] = up;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) up += s->warp[w];
+    v[1] = up;
+    v[0] = up - own + v[0];
+}
+
 struct Row {
     Shared *s;
     const float *l;          // this row
     unsigned begin, end;     // this warp's indices
+    unsigned cta_begin, cta_end, warp_span;
     unsigned rank, ranks;
+    bool vec;                // the row is 16-byte aligned
     int meeting, round;      // which of the alternating words and bucket sets is next
     float top, temperature, scale;
 
     // A token's weight, and that in units of 2^-40 (the rest of a unit is dropped).  scale: log2(e) / T.
-    __device__ __forceinline__ float weight(float x) const { return x == top ? 1.0f : exp2f(fmaxf(x - top, -3.402823466e38f) * scale); }
+    __device__ __forceinline__ float weight(float x) const { 
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf(x - top, -3.402823466e38f) * scale));
+        return x == top ? 1.0f : w;
+    }
     __device__ __forceinline__ static unsigned long long units(float w) {
         const uint32_t b = __float_as_uint(w);  // 0 <= w <= 1: 24 bits of mantissa, an exponent of at most 127
         return ((unsigned long long)((b & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (b >> 23), 63u);
     }
 
+    // f(index, logit) for every logit of the warp, and now and then for an index behind them with -inf.  One loop, whose
+    // loads alone differ (rows that are 16-byte aligned go by float4): the bodies are inlined eight times as it is.
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
-        unsigned i = begin + (threadIdx.x & 31);
-        for (; i + 224 < end; i += 256) {
+        const int lane = threadIdx.x & 31;
+        for (unsigned i0 = begin; i0 < end; i0 += 256) {
             float x[8];
+            if (vec) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = l[i + u * 32];
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned i = i0 + h * 128 + lane * 4;
+                    float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (i + 3 < end) {
+                        q = *reinterpret_cast<const float4 *>(l + i);
+                    } else {
+                        if (i < end) q.x = l[i];
+                        if (i + 1 < end) q.y = l[i + 1];
+                        if (i + 2 < end) q.z = l[i + 2];
+                    }
+                    x[4 * h] = q.x, x[4 * h + 1] = q.y, x[4 * h + 2] = q.z, x[4 * h + 3] = q.w;
+                }
+            } else {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) f(i + u * 32, x[u]);
+                for (int u = 0; u < 8; ++u) x[u] = i0 + u * 32 + lane < end ? l[i0 + u * 32 + lane] : -INFINITY;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) f(i0 + (vec ? (u >> 2) * 128 + lane * 4 + (u & 3) : u * 32 + lane), x[u]);
         }
-        for (; i < end; i += 32) f(i, l[i]);
     }
 
     // Every CTA's word to every CTA; `mine` is the same in all threads.
@@ -186,27 +228,21 @@ struct Row {
             if (before + part > want) break;
             before += part;
         }
-        if (owner == rank) {
-            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-            for (int k = 0; k < warp; ++k) before += s->warp[k];
-            if (before <= want && before + s->warp[warp] > want) {  // one warp
-                unsigned at = end;
-                for (unsigned i0 = begin; i0 < end; i0 += 32) {
-                    const unsigned i = i0 + lane;
-                    unsigned long long up = i < end ? f(i, l[i]) : 0;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const unsigned long long u = __shfl_up_sync(0xffffffffu, up, o);
-                        if (lane >= o) up += u;
-                    }
-                    const unsigned hit = __ballot_sync(0xffffffffu, before + up > want);
-                    if (hit) {
-                        at = i0 + __ffs(hit) - 1;
-                        break;
-                    }
-                    before += __shfl_sync(0xffffffffu, up, 31);
-                }
-                if (lane == 0) s->found = at;
+        if (owner == rank) {  // the warp whose part holds it, then all threads on that part, a few logits each
+            int warp = 0;
+            while (warp < SM_WARPS - 1 && before + s->warp[warp] <= want) before += s->warp[warp++];
+            const unsigned lo = min(cta_begin + warp * warp_span, cta_end), hi = min(lo + warp_span, cta_end);
+            const unsigned each_has = (hi - lo + SM_THREADS - 1) / SM_THREADS;
+            const unsigned from = min(lo + threadIdx.x * each_has, hi), to = min(from + each_has, hi);
+            unsigned long long v[2] = {0, 0};
+            for (unsigned i = from; i < to; ++i) v[0] += f(i, l[i]);
+            const unsigned long long own = v[0];
+            block_prefix(s, v);
+            unsigned long long upto = before + v[0] - own;
+            if (upto <= want && upto + own > want) {  // one thread
+                unsigned i = from;
+                while ((upto += f(i, l[i])) <= want) ++i;
+                s->found = i;
             }
         }
         cluster_meet();
@@ -316,24 +352,6 @@ struct Row {
     }
 };
 
-// A block's prefix sums of two values a thread (places 2t and 2t + 1): `v` becomes the sums up to and with each.
-__device__ __forceinline__ void block_prefix(Shared *s, unsigned long long (&v)[2]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned long long own = v[0] + v[1];
-    unsigned long long up = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long u = __shfl_up_sync(0xffffffffu, up, o);
-        if (lane >= o) up += u;
-    }
-    __syncthreads();
-    if (lane == 31) s->warp[warp] = up;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) up += s->warp[w];
-    v[1] = up;
-    v[0] = up - own + v[0];
-}
-
 // Sorts the first `n` (a power of two) of the list, largest first; all threads.
 __device__ __forceinline__ void sort_list(unsigned long long *x, unsigned n) {
     for (unsigned size = 2; size <= n; size <<= 1)
@@ -360,97 +378,114 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
     Shared *s = r.s;
     const float inv = __fdiv_rn(SM_PER_T, r.temperature);
     const bool by_mass = set.top_p < 1.0f;
-    auto bucket_of = [&](float x) {  // never falls as x falls; SM_BUCKETS: farther off than the buckets reach
-        const float d = x == r.top ? 0.0f : (r.top - x) * inv;
-        return d < (float)SM_BUCKETS ? (int)d : SM_BUCKETS;
+    auto distance = [&](float x) { return x == r.top ? 0.0f : (r.top - x) * inv; };  // in sixteenths of T; never falls as x falls
+    // Buckets: of one sixteenth up to 12 T, of a quarter up to 28 T, where a mass is less than a unit and counts as none; or 256
+    // in the place of one of those, [lo, hi).
+    float lo = 0.0f, hi = 4.0f * SM_BUCKETS - 3.0f * SM_FINE, per = 1.0f;
+    bool whole = true;
+    auto bucket = [&](float d) {  // -1: none
+        if (!(d >= lo && d < hi)) return -1;
+        const float t = (d - lo) * per;
+        return min(whole && t >= (float)SM_FINE ? SM_FINE + (int)((t - (float)SM_FINE) * 0.25f) : (int)t, SM_BUCKETS - 1);
     };
-    unsigned rest = 0;
-    unsigned long long rest_mass = 0;
-    r.each([&](unsigned, float x) {
-        if (key_of(x) <= KEY_NONE) return;
-        const int j = bucket_of(x);
-        if (j < SM_BUCKETS) {
-            atomicAdd(&s->count[j], 1u);
-            if (by_mass) atomicAdd(&s->mass[0][j], Row::units(r.weight(x)));
-        } else {
-            ++rest;
-            if (by_mass && set.k == 0) rest_mass += Row::units(r.weight(x));  // with top-k only the list's masses matter
-        }
-    });
-    const unsigned long long mine = r.block_sum(rest), mine_mass = r.block_sum(rest_mass);
-    if (threadIdx.x == 0) s->rest[0] = mine, s->rest[1] = mine_mass;
-    cluster_meet();
-    unsigned long long others = 0, others_mass = 0;
-    for (unsigned q = 0; q < r.ranks; ++q) {
-        others += ld_cluster_u64(&s->rest[0], q);
-        others_mass += ld_cluster_u64(&s->rest[1], q);
-    }
-    if (threadIdx.x < SM_BUCKETS) {
-        unsigned c = 0;
-        unsigned long long m = 0;
-        for (unsigned q = 0; q < r.ranks; ++q) {
-            c += ld_cluster_u32(&s->count[threadIdx.x], q);
-            if (by_mass) m += ld_cluster_u64(&s->mass[0][threadIdx.x], q);
-        }
-        s->all_count[threadIdx.x] = c;
-        s->all[threadIdx.x] = m;
-    }
-    __syncthreads();
-    // Sums up to and with each bucket; thread t has buckets 2t and 2t + 1.
-    unsigned long long counts[2] = {0, 0}, masses[2] = {0, 0};
-    if (threadIdx.x < SM_BUCKETS / 2) {
-        counts[0] = s->all_count[2 * threadIdx.x], counts[1] = s->all_count[2 * threadIdx.x + 1];
-        masses[0] = s->all[2 * threadIdx.x], masses[1] = s->all[2 * threadIdx.x + 1];
-    }
-    block_prefix(s, counts);
-    if (by_mass) block_prefix(s, masses);
-    __syncthreads();
-    if (threadIdx.x < SM_BUCKETS / 2) {
-        s->all_count[2 * threadIdx.x] = (unsigned)counts[0], s->all_count[2 * threadIdx.x + 1] = (unsigned)counts[1];
-        s->all[2 * threadIdx.x] = masses[0], s->all[2 * threadIdx.x + 1] = masses[1];
-    }
-    __syncthreads();
-    const unsigned long long tokens = s->all_count[SM_BUCKETS - 1] + others;
-    const unsigned long long mass = s->all[SM_BUCKETS - 1] + others_mass;
-    if (set.k > 0 && (unsigned long long)set.k >= tokens) {
-        if (by_mass && others) return -2;  // the mass beyond the buckets was not summed
-        set.k = 0;
-    }
-    // The last bucket that each setting can reach into.
     auto first = [&](auto &&reached) {  // of the buckets; SM_BUCKETS: none
-        int lo = 0, hi = SM_BUCKETS;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (reached(mid)) hi = mid;
-            else lo = mid + 1;
+        int from = 0, to = SM_BUCKETS;
+        while (from < to) {
+            const int mid = (from + to) / 2;
+            if (reached(mid)) to = mid;
+            else from = mid + 1;
         }
-        return lo;
+        return from;
     };
-    int last = SM_BUCKETS;
-    if (set.k > 0) last = first([&](int j) { return s->all_count[j] >= (unsigned)set.k; });
-    if (by_mass && set.k == 0) {
-        const double want = (double)set.top_p * (double)mass;
-        const int j = first([&](int q) { return (double)s->all[q] >= want; });
-        last = j < last ? j : last;
+    int last = 0;                                 // the bucket in which the settings' cut lies
+    unsigned from = 0, n = 0;                     // tokens before it, in it
+    unsigned long long mass = 0, mass_from = 0;   // of all tokens, of those before it
+    bool cut_only = false;                        // more than the list holds up to there: the list holds that bucket alone
+    double want = 0.0;
+#pragma unroll 1
+    for (int level = 0; level < 2; ++level) {
+        const int split = whole ? 20 : (lo < (float)SM_FINE ? 20 : 12);
+        r.each([&](unsigned, float x) {
+            const float d = distance(x);
+            const int j = bucket(d);
+            if (j < 0) return;
+            atomicAdd(&s->count[level][j], 1u);
+            if (by_mass) {  // in two halves: no carry for up to 4095 tokens of 2^40, or 2^20 of the light ones far off
+                const int at = whole && j >= SM_FINE ? 12 : split;
+                const unsigned long long v = Row::units(r.weight(x));
+                atomicAdd(&s->low[level][j], (unsigned)v & ((1u << at) - 1));
+                atomicAdd(&s->high[level][j], (unsigned)(v >> at));
+            }
+        });
+        cluster_meet();
+        unsigned long long counts[2] = {0, 0}, masses[2] = {0, 0};  // of buckets 2t and 2t + 1
+        if (threadIdx.x < SM_BUCKETS / 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int j = 2 * threadIdx.x + e, at = whole && j >= SM_FINE ? 12 : split;
+                for (unsigned q = 0; q < r.ranks; ++q) {
+                    const unsigned c = ld_cluster_u32(&s->count[level][j], q);
+                    counts[e] += c;
+                    if (!by_mass) continue;
+                    masses[e] += ((unsigned long long)ld_cluster_u32(&s->high[level][j], q) << at) + ld_cluster_u32(&s->low[level][j], q);
+                    if (at == 20 && c > 4095) s->kept = 1;  // a half may have run over
+                }
+            }
+        }
+        block_prefix(s, counts);
+        if (by_mass) block_prefix(s, masses);
+        if (threadIdx.x < SM_BUCKETS / 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s->all_count[2 * threadIdx.x + e] = (unsigned)counts[e], s->all[2 * threadIdx.x + e] = masses[e];
+        }
+        __syncthreads();
+        if (s->kept) return -2;
+        if (whole) {
+            mass = s->all[SM_BUCKETS - 1];
+            want = (double)set.top_p * (double)mass;
+            // what top-k would cut off behind the buckets has no mass
+            if (set.k > 0 && s->all_count[SM_BUCKETS - 1] < (unsigned)set.k) set.k = 0;
+        }
+        // Where each setting ends; top-p of a top-k needs the mass of all of these, so top-k's end comes first.
+        int end = SM_BUCKETS;
+        if (set.k > 0) end = first([&](int j) { return from + s->all_count[j] >= (unsigned)set.k; });
+        else if (by_mass) end = first([&](int j) { return (double)(mass_from + s->all[j]) >= want; });
+        bool cuts = end < SM_BUCKETS;
+        if (whole && set.min_p > 0.0f && !(by_mass && set.k > 0)) {
+            const float far = -logf(set.min_p) * SM_PER_T;
+            const int j = far < (float)SM_FINE ? (int)far + 1 : (far < hi - 8.0f ? SM_FINE + (int)((far - (float)SM_FINE) * 0.25f) + 1 : SM_BUCKETS);
+            if (j < end) end = j, cuts = false;
+        }
+        last = end;
+        if (whole && end < SM_BUCKETS && s->all_count[end] <= SM_LIST) {
+            n = s->all_count[end];
+            break;
+        }
+        cut_only = true;
+        if (!cuts) {  // all that min_p leaves, or all: the draw looks at the weights
+            n = 0;
+            break;
+        }
+        if (by_mass && set.k > 0) return -2;
+        n = s->all_count[end] - (end > 0 ? s->all_count[end - 1] : 0);
+        if (end > 0) from += s->all_count[end - 1], mass_from += s->all[end - 1];
+        if (n <= SM_LIST) break;
+        if (level == 1) return -2;
+        // once more, inside the bucket
+        lo = end < SM_FINE ? (float)end : (float)SM_FINE + 4.0f * (float)(end - SM_FINE);
+        hi = lo + (end < SM_FINE ? 1.0f : 4.0f);
+        per = (float)SM_BUCKETS / (hi - lo);
+        whole = false;
+        __syncthreads();  // all_count and all have been read
     }
-    if (set.min_p > 0.0f && !(by_mass && set.k > 0)) {  // top-p of a top-k needs the mass of all of these
-        const float far = -logf(set.min_p) * SM_PER_T;
-        if (far < (float)(SM_BUCKETS - 2) && (int)far + 1 < last) last = (int)far + 1;
-    }
-    if (last == SM_BUCKETS) return -2;
-    // More than the list holds up to there: then the last bucket alone, to find where the one setting that cuts ends in it.
-    const bool cut_only = s->all_count[last] > SM_LIST;
-    const unsigned from = cut_only && last > 0 ? s->all_count[last - 1] : 0;
-    const unsigned n = s->all_count[last] - from;
-    if (n > SM_LIST || (cut_only && by_mass && set.k > 0)) return -2;
-    const unsigned long long mass_from = cut_only && last > 0 ? s->all[last - 1] : 0;
 
-    r.each([&](unsigned i, float x) {
-        const uint32_t key = key_of(x);
-        const int j = bucket_of(x);
-        if (key > KEY_NONE && j <= last && (!cut_only || j == last))
-            st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key << 32 | (0xffffffffu - i));
-    });
+    if (!cut_only || n > 0) {
+        r.each([&](unsigned i, float x) {
+            const int j = bucket(distance(x));
+            if (j == last || (!cut_only && j >= 0 && j < last))
+                st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key_of(x) << 32 | (0xffffffffu - i));
+        });
+    }
     cluster_meet();
     if (cut_only) {
         // min_p needs no cut of its own: the draw looks at the weights
@@ -464,7 +499,7 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 upto[e] = w[e] = at + e < n && by_mass ? Row::units(r.weight(logit_of((uint32_t)(s->list[at + e] >> 32)))) : 0;
-            // nothing cuts in the bucket: min_p ended the buckets there
+            // nothing cuts: the draw goes by min_p alone
             if (threadIdx.x == 0) s->above = n ? s->list[n - 1] : (unsigned long long)(KEY_NONE + 1) << 32;
             block_prefix(s, upto);
             const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)mass) : 1ull;
@@ -478,7 +513,9 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
         cluster_meet();
         const unsigned long long cut = ld_cluster_u64(&s->above, 0);
         cluster_meet();  // rank 0 goes on to use the word
-        return (int)r.draw([&](unsigned i, float x) { return ((unsigned long long)key_of(x) << 32 | (0xffffffffu - i)) >= cut; }, set.min_p, set.u);
+        const float edge = logit_of((uint32_t)(cut >> 32));
+        const unsigned index = 0xffffffffu - (unsigned)cut;
+        return (int)r.draw([&](unsigned i, float x) { return x > edge || (x == edge && i <= index); }, set.min_p, set.u);
     }
     if (r.rank != 0) return 0;
 
@@ -532,11 +569,11 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
     __syncthreads();
     const unsigned long long sum = s->above;
     const double point = (double)set.u * (double)sum;
-    const unsigned long long want = point < (double)sum ? min((unsigned long long)point, sum - 1) : sum - 1;
+    const unsigned long long goal = point < (double)sum ? min((unsigned long long)point, sum - 1) : sum - 1;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const unsigned long long mass_here = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
-        if (mass_here && upto[e] > want && upto[e] - mass_here <= want) s->found = 0xffffffffu - (unsigned)(entry[e] >> 32);
+        if (mass_here && upto[e] > goal && upto[e] - mass_here <= goal) s->found = 0xffffffffu - (unsigned)(entry[e] >> 32);
     }
     __syncthreads();
     return (int)s->found;
@@ -593,15 +630,17 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r.ranks));
     const size_t row = blockIdx.x / r.ranks;
     r.l = p.logits + row * p.row_stride;
+    r.vec = (reinterpret_cast<uintptr_t>(r.l) & 15) == 0;
     r.meeting = r.round = 0;
     // indices of a CTA, and of a warp in it: contiguous, in whole 128-byte lines
-    const unsigned span = ((p.vocab + r.ranks - 1) / r.ranks + 31) & ~31u, warp_span = ((span + SM_WARPS - 1) / SM_WARPS + 31) & ~31u;
-    const unsigned cta_begin = min(r.rank * span, p.vocab), cta_end = min(cta_begin + span, p.vocab);
-    r.begin = min(cta_begin + (threadIdx.x >> 5) * warp_span, cta_end);
-    r.end = min(r.begin + warp_span, cta_end);
+    const unsigned span = ((p.vocab + r.ranks - 1) / r.ranks + 31) & ~31u;
+    r.warp_span = ((span + SM_WARPS - 1) / SM_WARPS + 31) & ~31u;
+    r.cta_begin = min(r.rank * span, p.vocab), r.cta_end = min(r.cta_begin + span, p.vocab);
+    r.begin = min(r.cta_begin + (threadIdx.x >> 5) * r.warp_span, r.cta_end);
+    r.end = min(r.begin + r.warp_span, r.cta_end);
     for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
-    if (threadIdx.x < SM_BUCKETS) sh.count[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sh.listed = 0;
+    for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.count[0][i] = sh.low[0][i] = sh.high[0][i] = 0;
+    if (threadIdx.x == 0) sh.listed = sh.kept = 0;
 
     // The largest logit (NaN is passed over).
     float top = -INFINITY;
@@ -614,12 +653,19 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     if (top_key <= KEY_NONE) {
         token = -1;  // no logit to choose
     } else if (!(t > 0.0f)) {
-        token = (int)r.locate([&](unsigned, float x) { return (unsigned long long)(key_of(x) == top_key); }, [](unsigned long long) { return 0ull; });
+        unsigned long long place = 0;  // the lowest index, as the largest of 2^32 - 1 - index
+        const float largest = logit_of(top_key);
+        r.each([&](unsigned i, float x) {
+            if (x == largest && 0xffffffffu - i > place) place = 0xffffffffu - i;
+        });
+        w = r.tell(r.block_max(place));
+        for (unsigned q = 0; q < r.ranks; ++q) place = max(place, ld_cluster_u64(w, q));
+        token = (int)(0xffffffffu - (unsigned)place);
     } else {
         r.top = logit_of(top_key);
         r.temperature = t;
         // finite, so that 0 * scale is 0; beside an infinite logit all others weigh nothing, whatever the temperature
-        r.scale = isinf(r.top) ? 3.402823466e38f : fminf(__fdiv_rn(1.44269504088896340736f, t), 3.402823466e38f);
+        r.scale = isinf(r.top) ? 3.402823466e38f : fminf(__fdiv_rn(1.44269504088896340736f, r.temperature), 3.402823466e38f);
         Settings set;
         set.k = p.top_k ? p.top_k[row] : 0;
         set.k = set.k > 0 && (unsigned)set.k < p.vocab ? set.k : 0;
@@ -630,7 +676,8 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         const float u = p.uniform[row];
         set.u = u > 0.0f ? u : 0.0f;
         token = -2;
-        if (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f) token = draw_from_list(r, set);
+        // (under a temperature near or at infinity -inf would get a weight there: the search asks for the key first)
+        if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(r, set);
         if (token == -2) {
             cluster_meet();  // the buckets have been read by everybody
             for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
