@@ -74,14 +74,14 @@ __device__ __forceinline__ unsigned long long ld_cluster_u64(const void *p, unsi
     uint32_t peer;
     unsigned long long v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer) : "memory");
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer));
     return v;
 }
 __device__ __forceinline__ unsigned ld_cluster_u32(const void *p, unsigned rank) {
     uint32_t peer;
     unsigned v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer));
     return v;
 }
 
@@ -167,13 +167,26 @@ struct Row {
         }
     }
 
-    // Every CTA's word to every CTA; `mine` is the same in all threads.
-    __device__ __forceinline__ const void *tell(unsigned long long mine) {
+    // Every CTA's word to every CTA; `mine` is the same in all threads.  Lane q gets rank q's word (0 behind the last rank): one
+    // look into another CTA's shared memory takes as long as eight side by side.
+    __device__ __forceinline__ unsigned long long tell(unsigned long long mine) {
         unsigned long long *w = &s->word[meeting & 1];
         ++meeting;
         if (threadIdx.x == 0) *w = mine;
         cluster_meet();
-        return w;
+        const unsigned q = threadIdx.x & 31;
+        return q < ranks ? ld_cluster_u64(w, q) : 0;
+    }
+    // Over the lanes of at most 8 ranks.
+    __device__ __forceinline__ static unsigned long long ranks_sum(unsigned long long v) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return __shfl_sync(0xffffffffu, v, 0);
+    }
+    __device__ __forceinline__ static unsigned long long ranks_max(unsigned long long v) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return __shfl_sync(0xffffffffu, v, 0);
     }
 
     __device__ __forceinline__ unsigned long long block_max(unsigned long long v) {
@@ -201,14 +214,20 @@ struct Row {
         for (int w = 0; w < SM_WARPS; ++w) v += s->warp[w];
         return v;
     }
+    // The sum of f(rank), whose looks are on their way together.
+    template <typename F>
+    __device__ __forceinline__ unsigned long long ranks_total(F &&f) const {
+        unsigned long long v[8];
+#pragma unroll
+        for (unsigned q = 0; q < 8; ++q) v[q] = q < ranks ? f(q) : 0;
+        return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+
     template <typename F>
     __device__ __forceinline__ unsigned long long total(F &&f) {
         unsigned long long v = 0;
         each([&](unsigned i, float x) { v += f(i, x); });
-        const void *w = tell(block_sum(v));
-        v = 0;
-        for (unsigned r = 0; r < ranks; ++r) v += ld_cluster_u64(w, r);
-        return v;
+        return ranks_sum(tell(block_sum(v)));
     }
 
     // The first index at which the running sum of f, in index order, exceeds goal(sum of all f); all CTAs learn it.
@@ -217,17 +236,16 @@ struct Row {
         unsigned long long v = 0;
         each([&](unsigned i, float x) { v += f(i, x); });
         const unsigned long long mine = block_sum(v);
-        const void *w = tell(mine);
-        unsigned long long sum = 0, before = 0;
-        for (unsigned r = 0; r < ranks; ++r) sum += ld_cluster_u64(w, r);
-        const unsigned long long want = goal(sum);
-        unsigned owner = 0;
-        for (unsigned r = 0; r < ranks; ++r) {
-            const unsigned long long part = ld_cluster_u64(w, r);
-            owner = r;
-            if (before + part > want) break;
-            before += part;
+        const unsigned long long part = tell(mine);
+        const unsigned long long want = goal(ranks_sum(part));
+        unsigned long long upto = part;  // of the ranks up to and with this lane's
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int)(threadIdx.x & 31) >= o) upto += u;
         }
+        const unsigned owner = __ffs(__ballot_sync(0xffffffffu, upto > want)) - 1;
+        unsigned long long before = __shfl_sync(0xffffffffu, upto - part, (int)owner);
         if (owner == rank) {  // the warp whose part holds it, then all threads on that part, a few logits each
             int warp = 0;
             while (warp < SM_WARPS - 1 && before + s->warp[warp] <= want) before += s->warp[warp++];
@@ -238,10 +256,10 @@ struct Row {
             for (unsigned i = from; i < to; ++i) v[0] += f(i, l[i]);
             const unsigned long long own = v[0];
             block_prefix(s, v);
-            unsigned long long upto = before + v[0] - own;
-            if (upto <= want && upto + own > want) {  // one thread
+            unsigned long long run = before + v[0] - own;
+            if (run <= want && run + own > want) {  // one thread
                 unsigned i = from;
-                while ((upto += f(i, l[i])) <= want) ++i;
+                while ((run += f(i, l[i])) <= want) ++i;
                 s->found = i;
             }
         }
@@ -298,9 +316,7 @@ struct Row {
             });
             cluster_meet();
             if (threadIdx.x < SM_BUCKETS) {
-                unsigned long long v = 0;
-                for (unsigned r = 0; r < ranks; ++r) v += ld_cluster_u64(&set[threadIdx.x], r);
-                s->all[threadIdx.x] = v;
+                s->all[threadIdx.x] = ranks_total([&](unsigned q) { return ld_cluster_u64(&set[threadIdx.x], q); });
                 s->mass[(round + 1) & 1][threadIdx.x] = 0;  // its readers passed the meeting
             }
             ++round;
@@ -354,9 +370,12 @@ struct Row {
 
 // Sorts the first `n` (a power of two) of the list, largest first; all threads.
 __device__ __forceinline__ void sort_list(unsigned long long *x, unsigned n) {
+    const bool one_warp = n <= 64;  // meets itself without a barrier of the CTA
+    __syncthreads();
     for (unsigned size = 2; size <= n; size <<= 1)
         for (unsigned gap = size >> 1; gap > 0; gap >>= 1) {
-            __syncthreads();
+            if (one_warp) __syncwarp();
+            else __syncthreads();
             for (unsigned i = threadIdx.x; i < n / 2; i += SM_THREADS) {
                 const unsigned lo = ((i & ~(gap - 1)) << 1) | (i & (gap - 1)), hi = lo | gap;
                 const unsigned long long a = x[lo], b = x[hi];
@@ -423,12 +442,16 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int j = 2 * threadIdx.x + e, at = whole && j >= SM_FINE ? 12 : split;
-                for (unsigned q = 0; q < r.ranks; ++q) {
+                unsigned most = 0;
+                counts[e] = r.ranks_total([&](unsigned q) {
                     const unsigned c = ld_cluster_u32(&s->count[level][j], q);
-                    counts[e] += c;
-                    if (!by_mass) continue;
-                    masses[e] += ((unsigned long long)ld_cluster_u32(&s->high[level][j], q) << at) + ld_cluster_u32(&s->low[level][j], q);
-                    if (at == 20 && c > 4095) s->kept = 1;  // a half may have run over
+                    most = max(most, c);
+                    return (unsigned long long)c;
+                });
+                if (by_mass) {
+                    masses[e] = (r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->high[level][j], q); }) << at) +
+                                r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->low[level][j], q); });
+                    if (at == 20 && most > 4095) s->kept = 1;  // a half may have run over
                 }
             }
         }
@@ -645,9 +668,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     // The largest logit (NaN is passed over).
     float top = -INFINITY;
     r.each([&](unsigned, float x) { top = fmaxf(top, x); });
-    uint32_t top_key = 0;
-    const void *w = r.tell(r.block_max(key_of(top)));
-    for (unsigned q = 0; q < r.ranks; ++q) top_key = max(top_key, (uint32_t)ld_cluster_u64(w, q));
+    const uint32_t top_key = (uint32_t)Row::ranks_max(r.tell(r.block_max(key_of(top))));
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     int token;
     if (top_key <= KEY_NONE) {
@@ -658,8 +679,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         r.each([&](unsigned i, float x) {
             if (x == largest && 0xffffffffu - i > place) place = 0xffffffffu - i;
         });
-        w = r.tell(r.block_max(place));
-        for (unsigned q = 0; q < r.ranks; ++q) place = max(place, ld_cluster_u64(w, q));
+        place = Row::ranks_max(r.tell(r.block_max(place)));
         token = (int)(0xffffffffu - (unsigned)place);
     } else {
         r.top = logit_of(top_key);
