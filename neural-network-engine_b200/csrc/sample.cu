@@ -11,9 +11,10 @@
 // other's shared memory: the row's later passes come from L1, and nothing of it goes through global memory or a
 // second launch.
 //
-// Three passes where the settings leave few tokens, as they nearly always do: the maximum; counts and masses by distance from
-// it, in 256 buckets of T / 16 and T / 4, which show up to which bucket the settings can reach; and the tokens up to that bucket, at most 1024,
-// into a list in the first CTA's shared memory.  That CTA sorts them, cuts the list and draws.
+// Two or three passes where the settings leave few tokens, as they nearly always do: the maximum; for top-p, counts and masses by
+// distance from it, in 256 buckets of T / 16 and T / 4, which show up to which bucket the settings can reach (top-k's reach is
+// bounded by the threads' own maxima, min-p's is known); and the tokens up to there, at most 1024, into a list in the first CTA's
+// shared memory.  That CTA orders them, cuts the list and draws.
 // Where more are left and one setting cuts them, the list holds the bucket of the cut (or, a pass more, a 256th of it), and two passes
 // draw from what is above it.
 // Else nothing is sorted: a logit's bits, made monotone, are its key; top-k and top-p are each a
@@ -368,20 +369,40 @@ struct Row {
     }
 };
 
-// Sorts the first `n` (a power of two) of the list, largest first; all threads.
-__device__ __forceinline__ void sort_list(unsigned long long *x, unsigned n) {
-    const bool one_warp = n <= 64;  // meets itself without a barrier of the CTA
+// Puts the first n (at most SM_LIST, all different and not 0) of the list in order, largest first; all threads.  Few: each
+// counts what is larger than its two (100: 1000 cycles, where a sorting network's barriers take 6000).  Above 384 the counting
+// would keep all warps busy for n rounds (1000: 36000 cycles) and the network is the shorter.
+__device__ __forceinline__ void order_list(Shared *s, unsigned n) {
     __syncthreads();
-    for (unsigned size = 2; size <= n; size <<= 1)
-        for (unsigned gap = size >> 1; gap > 0; gap >>= 1) {
-            if (one_warp) __syncwarp();
-            else __syncthreads();
-            for (unsigned i = threadIdx.x; i < n / 2; i += SM_THREADS) {
-                const unsigned lo = ((i & ~(gap - 1)) << 1) | (i & (gap - 1)), hi = lo | gap;
-                const unsigned long long a = x[lo], b = x[hi];
-                if ((a < b) == ((lo & size) == 0)) x[lo] = b, x[hi] = a;
+    if (n <= 384) {
+        const unsigned at = 2 * threadIdx.x;
+        const unsigned long long a = at < n ? s->list[at] : 0, b = at + 1 < n ? s->list[at + 1] : 0;
+        unsigned ra = 0, rb = 0;
+        if (at < n) {
+#pragma unroll 4
+            for (unsigned j = 0; j < n; ++j) {
+                const unsigned long long x = s->list[j];
+                ra += x > a, rb += x > b;
             }
         }
+        __syncthreads();
+        if (at < n) s->list[ra] = a;
+        if (at + 1 < n) s->list[rb] = b;
+    } else {
+        unsigned size = 512;
+        while (size < n) size <<= 1;
+        for (unsigned i = n + threadIdx.x; i < size; i += SM_THREADS) s->list[i] = 0;
+        for (unsigned len = 2; len <= size; len <<= 1)
+            for (unsigned gap = len >> 1; gap > 0; gap >>= 1) {
+                __syncthreads();
+                const unsigned i = threadIdx.x;
+                if (i < size / 2) {
+                    const unsigned lo = ((i & ~(gap - 1)) << 1) | (i & (gap - 1)), hi = lo | gap;
+                    const unsigned long long x = s->list[lo], y = s->list[hi];
+                    if ((x < y) == ((lo & len) == 0)) s->list[lo] = y, s->list[hi] = x;
+                }
+            }
+    }
     __syncthreads();
 }
 
@@ -392,18 +413,20 @@ struct Settings {
     float u;
 };
 
-// The token, where the settings leave at most SM_LIST, or -2.  All CTAs return the same.
-__device__ __noinline__ int draw_from_list(Row &r, Settings set) {
+// The token (rank 0's return value), where the list holds what is needed for it, or -2 in all CTAs.  `mine`: the largest logit
+// that this thread has seen.
+__device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
     Shared *s = r.s;
     const float inv = __fdiv_rn(SM_PER_T, r.temperature);
+    if (!(inv < 1e30f) || isinf(r.top)) return -2;  // distances need numbers to be measured in
     const bool by_mass = set.top_p < 1.0f;
-    auto distance = [&](float x) { return x == r.top ? 0.0f : (r.top - x) * inv; };  // in sixteenths of T; never falls as x falls
+    auto distance = [&](float x) { return (r.top - x) * inv; };  // in sixteenths of T; never falls as x falls
     // Buckets: of one sixteenth up to 12 T, of a quarter up to 28 T, where a mass is less than a unit and counts as none; or 256
     // in the place of one of those, [lo, hi).
-    float lo = 0.0f, hi = 4.0f * SM_BUCKETS - 3.0f * SM_FINE, per = 1.0f;
+    constexpr float END = 4.0f * SM_BUCKETS - 3.0f * SM_FINE;
+    float lo = 0.0f, hi = END, per = 1.0f;
     bool whole = true;
-    auto bucket = [&](float d) {  // -1: none
-        if (!(d >= lo && d < hi)) return -1;
+    auto bucket = [&](float d) {  // of a distance in [lo, hi)
         const float t = (d - lo) * per;
         return min(whole && t >= (float)SM_FINE ? SM_FINE + (int)((t - (float)SM_FINE) * 0.25f) : (int)t, SM_BUCKETS - 1);
     };
@@ -416,150 +439,198 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
         }
         return from;
     };
-    int last = 0;                                 // the bucket in which the settings' cut lies
-    unsigned from = 0, n = 0;                     // tokens before it, in it
-    unsigned long long mass = 0, mass_from = 0;   // of all tokens, of those before it
-    bool cut_only = false;                        // more than the list holds up to there: the list holds that bucket alone
-    double want = 0.0;
-#pragma unroll 1
-    for (int level = 0; level < 2; ++level) {
-        const int split = whole ? 20 : (lo < (float)SM_FINE ? 20 : 12);
-        r.each([&](unsigned, float x) {
-            const float d = distance(x);
-            const int j = bucket(d);
-            if (j < 0) return;
-            atomicAdd(&s->count[level][j], 1u);
-            if (by_mass) {  // in two halves: no carry for up to 4095 tokens of 2^40, or 2^20 of the light ones far off
-                const int at = whole && j >= SM_FINE ? 12 : split;
-                const unsigned long long v = Row::units(r.weight(x));
-                atomicAdd(&s->low[level][j], (unsigned)v & ((1u << at) - 1));
-                atomicAdd(&s->high[level][j], (unsigned)(v >> at));
-            }
-        });
+    // The cluster's counts (and masses) up to and with each bucket, of a set of buckets that all CTAs have filled.
+    auto gather_buckets = [&](int level, int split, bool masses) {
         cluster_meet();
-        unsigned long long counts[2] = {0, 0}, masses[2] = {0, 0};  // of buckets 2t and 2t + 1
-        if (threadIdx.x < SM_BUCKETS / 2) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = 2 * threadIdx.x + e, at = whole && j >= SM_FINE ? 12 : split;
-                unsigned most = 0;
-                counts[e] = r.ranks_total([&](unsigned q) {
-                    const unsigned c = ld_cluster_u32(&s->count[level][j], q);
-                    most = max(most, c);
-                    return (unsigned long long)c;
-                });
-                if (by_mass) {
-                    masses[e] = (r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->high[level][j], q); }) << at) +
-                                r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->low[level][j], q); });
-                    if (at == 20 && most > 4095) s->kept = 1;  // a half may have run over
-                }
-            }
-        }
-        block_prefix(s, counts);
-        if (by_mass) block_prefix(s, masses);
-        if (threadIdx.x < SM_BUCKETS / 2) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) s->all_count[2 * threadIdx.x + e] = (unsigned)counts[e], s->all[2 * threadIdx.x + e] = masses[e];
+        const unsigned j = threadIdx.x & (SM_BUCKETS - 1);
+        const int at = whole && (int)j >= SM_FINE ? 12 : split;
+        if (threadIdx.x < SM_BUCKETS) {
+            unsigned most = 0;
+            s->all_count[j] = (unsigned)r.ranks_total([&](unsigned q) {
+                const unsigned c = ld_cluster_u32(&s->count[level][j], q);
+                most = max(most, c);
+                return (unsigned long long)c;
+            });
+            if (masses && at == 20 && most > 4095) s->kept = 1;  // a half may have run over
+        } else if (masses) {
+            s->all[j] = (r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->high[level][j], q); }) << at) +
+                        r.ranks_total([&](unsigned q) { return (unsigned long long)ld_cluster_u32(&s->low[level][j], q); });
         }
         __syncthreads();
-        if (s->kept) return -2;
-        if (whole) {
-            mass = s->all[SM_BUCKETS - 1];
-            want = (double)set.top_p * (double)mass;
-            // what top-k would cut off behind the buckets has no mass
-            if (set.k > 0 && s->all_count[SM_BUCKETS - 1] < (unsigned)set.k) set.k = 0;
-        }
-        // Where each setting ends; top-p of a top-k needs the mass of all of these, so top-k's end comes first.
-        int end = SM_BUCKETS;
-        if (set.k > 0) end = first([&](int j) { return from + s->all_count[j] >= (unsigned)set.k; });
-        else if (by_mass) end = first([&](int j) { return (double)(mass_from + s->all[j]) >= want; });
-        bool cuts = end < SM_BUCKETS;
-        if (whole && set.min_p > 0.0f && !(by_mass && set.k > 0)) {
-            const float far = -logf(set.min_p) * SM_PER_T;
-            const int j = far < (float)SM_FINE ? (int)far + 1 : (far < hi - 8.0f ? SM_FINE + (int)((far - (float)SM_FINE) * 0.25f) + 1 : SM_BUCKETS);
-            if (j < end) end = j, cuts = false;
-        }
-        last = end;
-        if (whole && end < SM_BUCKETS && s->all_count[end] <= SM_LIST) {
-            n = s->all_count[end];
-            break;
-        }
-        cut_only = true;
-        if (!cuts) {  // all that min_p leaves, or all: the draw looks at the weights
-            n = 0;
-            break;
-        }
-        if (by_mass && set.k > 0) return -2;
-        n = s->all_count[end] - (end > 0 ? s->all_count[end - 1] : 0);
-        if (end > 0) from += s->all_count[end - 1], mass_from += s->all[end - 1];
-        if (n <= SM_LIST) break;
-        if (level == 1) return -2;
-        // once more, inside the bucket
-        lo = end < SM_FINE ? (float)end : (float)SM_FINE + 4.0f * (float)(end - SM_FINE);
-        hi = lo + (end < SM_FINE ? 1.0f : 4.0f);
-        per = (float)SM_BUCKETS / (hi - lo);
-        whole = false;
-        __syncthreads();  // all_count and all have been read
-    }
-
-    if (!cut_only || n > 0) {
-        r.each([&](unsigned i, float x) {
-            const int j = bucket(distance(x));
-            if (j == last || (!cut_only && j >= 0 && j < last))
-                st_cluster_u64(&s->list[add_cluster_u32(&s->listed, 0, 1)], 0, (unsigned long long)key_of(x) << 32 | (0xffffffffu - i));
-        });
-    }
-    cluster_meet();
-    if (cut_only) {
-        // min_p needs no cut of its own: the draw looks at the weights
-        if (r.rank == 0) {
-            unsigned size = 2;
-            while (size < n) size <<= 1;
-            for (unsigned i = n + threadIdx.x; i < size; i += SM_THREADS) s->list[i] = 0;
-            sort_list(s->list, size);
-            const unsigned at = 2 * threadIdx.x;
-            unsigned long long w[2], upto[2];
+        if (threadIdx.x < 64 && (threadIdx.x < 32 || masses)) {  // one warp the counts, one the masses: eight buckets a lane
+            constexpr int N = SM_BUCKETS / 32;
+            const int lane = threadIdx.x & 31;
+            const bool m = threadIdx.x >= 32;
+            unsigned long long v[N], up = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                upto[e] = w[e] = at + e < n && by_mass ? Row::units(r.weight(logit_of((uint32_t)(s->list[at + e] >> 32)))) : 0;
-            // nothing cuts: the draw goes by min_p alone
-            if (threadIdx.x == 0) s->above = n ? s->list[n - 1] : (unsigned long long)(KEY_NONE + 1) << 32;
-            block_prefix(s, upto);
-            const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)mass) : 1ull;
+            for (int k = 0; k < N; ++k) up += m ? s->all[lane * N + k] : s->all_count[lane * N + k], v[k] = up;
+            unsigned long long before = up;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bool cuts = set.k > 0 ? from + at + e + 1 == (unsigned)set.k
-                                            : by_mass && w[e] && mass_from + upto[e] - w[e] < target && mass_from + upto[e] >= target;
-                if (at + e < n && cuts) s->above = s->list[at + e];
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long u = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += u;
+            }
+            before -= up;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if (m) s->all[lane * N + k] = before + v[k];
+                else s->all_count[lane * N + k] = (unsigned)(before + v[k]);
             }
         }
+        __syncthreads();
+    };
+    // Tokens nearer than `edge` but not than `near` into rank 0's list, as far as it holds them; their number.
+    auto gather_tokens = [&](float near, float edge, auto &&in) {
+        r.each([&](unsigned i, float x) {
+            const float d = distance(x);
+            if (d < edge && d >= near && in(d)) {
+                const unsigned slot = add_cluster_u32(&s->listed, 0, 1);
+                if (slot < SM_LIST) st_cluster_u64(&s->list[slot], 0, (unsigned long long)key_of(x) << 32 | (0xffffffffu - i));
+            }
+        });
         cluster_meet();
-        const unsigned long long cut = ld_cluster_u64(&s->above, 0);
-        cluster_meet();  // rank 0 goes on to use the word
-        const float edge = logit_of((uint32_t)(cut >> 32));
-        const unsigned index = 0xffffffffu - (unsigned)cut;
-        return (int)r.draw([&](unsigned i, float x) { return x > edge || (x == edge && i <= index); }, set.min_p, set.u);
+        return ld_cluster_u32(&s->listed, 0);
+    };
+    const float far = set.min_p > 0.0f ? -logf(set.min_p) * SM_PER_T + 1.0f : END;  // what is farther min_p leaves out
+
+    unsigned n = 0;
+    bool listed = false;
+    unsigned long long mass = 0;
+    if (set.k > 0) {
+        // The k-th largest of the threads' maxima is at most the k-th largest logit: all that top-k can keep is nearer than
+        // that maximum's bucket ends.
+        const float d = distance(mine);
+        if (d < END) atomicAdd(&s->count[2][bucket(d)], 1u);
+        gather_buckets(2, 20, false);
+        const int end = first([&](int j) { return s->all_count[j] >= (unsigned)set.k; });
+        if (end < SM_BUCKETS) {
+            float edge = end < SM_FINE ? (float)(end + 1) : (float)SM_FINE + 4.0f * (float)(end + 1 - SM_FINE);
+            if (!by_mass) edge = fminf(edge, far);  // top-p of a top-k needs the mass of all of these
+            n = gather_tokens(0.0f, edge, [](float) { return true; });
+            listed = n <= SM_LIST;
+        }
+    } else if (!by_mass && far < END) {
+        n = gather_tokens(0.0f, far, [](float) { return true; });
+        listed = n <= SM_LIST;
+        if (!listed) {
+            cluster_meet();  // the count has been read by everybody
+            return (int)r.draw([&](unsigned, float x) { return x > -INFINITY; }, set.min_p, set.u);
+        }
+    }
+    if (!listed) {
+        // By counts and masses of all tokens' buckets, and of those inside a crowded one.
+        if (n > 0) {
+            cluster_meet();
+            if (threadIdx.x == 0) s->listed = 0;
+        }
+        int last = 0;                        // the bucket in which the settings' cut lies
+        unsigned from = 0;                   // tokens before it
+        unsigned long long mass_from = 0;    // their mass
+        double want = 0.0;
+        bool cut_only = false;               // more than the list holds up to there: the list holds that bucket alone
+#pragma unroll 1
+        for (int level = 0; level < 2; ++level) {
+            const int split = whole ? 20 : (lo < (float)SM_FINE ? 20 : 12);
+            r.each([&](unsigned, float x) {
+                const float d = distance(x);
+                if (!(d >= lo && d < hi)) return;
+                const int j = bucket(d);
+                atomicAdd(&s->count[level][j], 1u);
+                if (by_mass) {  // in two halves: no carry for up to 4095 tokens of 2^40, or 2^20 of the light ones far off
+                    const int at = whole && j >= SM_FINE ? 12 : split;
+                    const unsigned long long v = Row::units(r.weight(x));
+                    atomicAdd(&s->low[level][j], (unsigned)v & ((1u << at) - 1));
+                    atomicAdd(&s->high[level][j], (unsigned)(v >> at));
+                }
+            });
+            gather_buckets(level, split, by_mass);
+            if (s->kept) return -2;
+            if (whole) {
+                mass = s->all[SM_BUCKETS - 1];
+                want = (double)set.top_p * (double)mass;
+                // what top-k would cut off behind the buckets has no mass
+                if (set.k > 0 && s->all_count[SM_BUCKETS - 1] < (unsigned)set.k) set.k = 0;
+            }
+            // Where each setting ends; top-p of a top-k needs the mass of all of these, so top-k's end comes first.
+            int end = SM_BUCKETS;
+            if (set.k > 0) end = first([&](int j) { return from + s->all_count[j] >= (unsigned)set.k; });
+            else if (by_mass) end = first([&](int j) { return (double)(mass_from + s->all[j]) >= want; });
+            bool cuts = end < SM_BUCKETS;
+            if (whole && far < END && !(by_mass && set.k > 0)) {
+                const int j = bucket(far);
+                if (j < end) end = j, cuts = false;
+            }
+            last = end;
+            if (whole && end < SM_BUCKETS && s->all_count[end] <= SM_LIST) {
+                n = s->all_count[end];
+                break;
+            }
+            cut_only = true;
+            if (!cuts) {  // all that min_p leaves, or all: the draw looks at the weights
+                n = 0;
+                break;
+            }
+            if (by_mass && set.k > 0) return -2;
+            n = s->all_count[end] - (end > 0 ? s->all_count[end - 1] : 0);
+            if (end > 0) from += s->all_count[end - 1], mass_from += s->all[end - 1];
+            if (n <= SM_LIST) break;
+            if (level == 1) return -2;
+            // once more, inside the bucket
+            lo = end < SM_FINE ? (float)end : (float)SM_FINE + 4.0f * (float)(end - SM_FINE);
+            hi = lo + (end < SM_FINE ? 1.0f : 4.0f);
+            per = (float)SM_BUCKETS / (hi - lo);
+            whole = false;
+            __syncthreads();  // all_count and all have been read
+        }
+        if (cut_only) {
+            float edge = -3.402823466e38f;  // without a cut: all
+            unsigned index = 0xffffffffu;
+            if (n > 0) {
+                gather_tokens(lo, hi, [&](float d) { return bucket(d) == last; });
+                if (r.rank == 0) {
+                    order_list(s, n);
+                    const unsigned at = 2 * threadIdx.x;
+                    unsigned long long w[2], upto[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        upto[e] = w[e] = at + e < n && by_mass ? Row::units(r.weight(logit_of((uint32_t)(s->list[at + e] >> 32)))) : 0;
+                    if (threadIdx.x == 0) s->above = s->list[n - 1];
+                    block_prefix(s, upto);
+                    const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)mass) : 1ull;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool here = set.k > 0 ? from + at + e + 1 == (unsigned)set.k
+                                                    : w[e] && mass_from + upto[e] - w[e] < target && mass_from + upto[e] >= target;
+                        if (at + e < n && here) s->above = s->list[at + e];
+                    }
+                }
+                cluster_meet();
+                const unsigned long long cut = ld_cluster_u64(&s->above, 0);
+                edge = logit_of((uint32_t)(cut >> 32));
+                index = 0xffffffffu - (unsigned)cut;
+                cluster_meet();  // rank 0 goes on to use the word
+            }
+            return (int)r.draw([&](unsigned i, float x) { return x > edge || (x == edge && i <= index); }, set.min_p, set.u);
+        }
+        const float edge = last < SM_FINE ? (float)(last + 1) : (float)SM_FINE + 4.0f * (float)(last + 1 - SM_FINE);
+        gather_tokens(0.0f, edge, [](float) { return true; });
     }
     if (r.rank != 0) return 0;
 
-    unsigned size = 2;
-    while (size < n) size <<= 1;
-    for (unsigned i = n + threadIdx.x; i < size; i += SM_THREADS) s->list[i] = 0;
-    sort_list(s->list, size);
+    order_list(s, n);
+    if (set.k > 0 && (unsigned)set.k > n) set.k = 0;  // min_p's end came first, and what is farther it leaves out
     const unsigned at = 2 * threadIdx.x;
     unsigned long long entry[2], w[2], upto[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         entry[e] = at + e < n ? s->list[at + e] : 0;
-        const float x = logit_of((uint32_t)(entry[e] >> 32));
-        w[e] = at + e < n ? Row::units(r.weight(x)) : 0;
+        w[e] = at + e < n ? Row::units(r.weight(logit_of((uint32_t)(entry[e] >> 32)))) : 0;
         upto[e] = w[e];
     }
     block_prefix(s, upto);
-    const unsigned most = set.k > 0 ? (unsigned)set.k : SM_LIST;  // top-k: places below this (n >= k)
-    __syncthreads();
+    const unsigned most = set.k > 0 ? (unsigned)set.k : SM_LIST;  // top-k: places below this
+    if (set.k > 0 && at <= most - 1 && most - 1 < at + 2) s->above = (most - 1) & 1 ? upto[1] : upto[0];
     if (threadIdx.x == 0) s->kept = 0;
-    if (set.k > 0 && at <= most - 1 && most - 1 < at + 2) s->above = upto[(most - 1) & 1];
     __syncthreads();
     const unsigned long long of = set.k > 0 ? s->above : mass;
     const unsigned long long target = set.top_p > 0.0f ? (unsigned long long)ceil((double)set.top_p * (double)of) : 1ull;
@@ -572,20 +643,19 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
         if (set.min_p > 0.0f) in = in && r.weight(logit_of((uint32_t)(entry[e] >> 32))) >= set.min_p;
         keeps += in;
     }
-    atomicAdd(&s->kept, keeps);
+    keeps = __reduce_add_sync(0xffffffffu, keeps);
+    if ((threadIdx.x & 31) == 0 && keeps) atomicAdd(&s->kept, keeps);
     __syncthreads();
     const unsigned kept = s->kept;  // the first places: each condition holds up to some place
-    // In index order: sorted by index, falling, from the back.
-    unsigned ksize = 2;
-    while (ksize < kept) ksize <<= 1;
+    // In index order: (2^32 - 1 - index, key), largest first.
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-        if (at + e < ksize) s->list[at + e] = at + e < kept ? (entry[e] << 32) | (entry[e] >> 32) : 0;  // (2^32 - 1 - index, key): low indices first
-    sort_list(s->list, ksize);
+        if (at + e < kept) s->list[at + e] = (entry[e] << 32) | (entry[e] >> 32);
+    order_list(s, kept);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         entry[e] = at + e < kept ? s->list[at + e] : 0;
-        upto[e] = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
+        upto[e] = w[e] = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
     }
     block_prefix(s, upto);
     if (threadIdx.x == SM_THREADS - 1) s->above = upto[1];
@@ -594,10 +664,8 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set) {
     const double point = (double)set.u * (double)sum;
     const unsigned long long goal = point < (double)sum ? min((unsigned long long)point, sum - 1) : sum - 1;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const unsigned long long mass_here = at + e < kept ? Row::units(r.weight(logit_of((uint32_t)entry[e]))) : 0;
-        if (mass_here && upto[e] > goal && upto[e] - mass_here <= goal) s->found = 0xffffffffu - (unsigned)(entry[e] >> 32);
-    }
+    for (int e = 0; e < 2; ++e)
+        if (w[e] && upto[e] > goal && upto[e] - w[e] <= goal) s->found = 0xffffffffu - (unsigned)(entry[e] >> 32);
     __syncthreads();
     return (int)s->found;
 }
@@ -665,11 +733,21 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.count[0][i] = sh.low[0][i] = sh.high[0][i] = 0;
     if (threadIdx.x == 0) sh.listed = sh.kept = 0;
 
+    // Settings now: their latency passes under the first pass.
+    const float t = p.temperature ? p.temperature[row] : 1.0f, u = p.uniform[row];
+    Settings set;
+    set.k = p.top_k ? p.top_k[row] : 0;
+    set.top_p = p.top_p ? p.top_p[row] : 1.0f;
+    set.min_p = p.min_p ? p.min_p[row] : 0.0f;
+    set.k = set.k > 0 && (unsigned)set.k < p.vocab ? set.k : 0;
+    set.top_p = set.top_p < 1.0f ? set.top_p : 1.0f;  // NaN: off
+    set.min_p = set.min_p > 0.0f ? fminf(set.min_p, 1.0f) : 0.0f;
+    set.u = u > 0.0f ? u : 0.0f;
+
     // The largest logit (NaN is passed over).
     float top = -INFINITY;
     r.each([&](unsigned, float x) { top = fmaxf(top, x); });
     const uint32_t top_key = (uint32_t)Row::ranks_max(r.tell(r.block_max(key_of(top))));
-    const float t = p.temperature ? p.temperature[row] : 1.0f;
     int token;
     if (top_key <= KEY_NONE) {
         token = -1;  // no logit to choose
@@ -686,18 +764,9 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         r.temperature = t;
         // finite, so that 0 * scale is 0; beside an infinite logit all others weigh nothing, whatever the temperature
         r.scale = isinf(r.top) ? 3.402823466e38f : fminf(__fdiv_rn(1.44269504088896340736f, r.temperature), 3.402823466e38f);
-        Settings set;
-        set.k = p.top_k ? p.top_k[row] : 0;
-        set.k = set.k > 0 && (unsigned)set.k < p.vocab ? set.k : 0;
-        set.top_p = p.top_p ? p.top_p[row] : 1.0f;
-        set.top_p = set.top_p < 1.0f ? set.top_p : 1.0f;  // NaN: off
-        set.min_p = p.min_p ? p.min_p[row] : 0.0f;
-        set.min_p = set.min_p > 0.0f ? fminf(set.min_p, 1.0f) : 0.0f;
-        const float u = p.uniform[row];
-        set.u = u > 0.0f ? u : 0.0f;
         token = -2;
         // (under a temperature near or at infinity -inf would get a weight there: the search asks for the key first)
-        if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(r, set);
+        if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(r, set, top);
         if (token == -2) {
             cluster_meet();  // the buckets have been read by everybody
             for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
