@@ -28,7 +28,12 @@ int check_cache(const nne_kv_cache *c) {
 namespace {
 
 constexpr int AP_WARPS = 8;  // heads a CTA works on at a time
-constexpr int AP_BATCH = 2;  // of those, how many a warp has loads for on their way
+// Of those, how many a warp has loads for on their way.  (Six, with the registers they take, leave fewer CTAs an SM to
+// cover the chain index -> table -> store: 6001 tokens 71 us instead of 55.)
+constexpr int AP_BATCH = 2;
+// CTAs an SM: eight, at 32 registers a thread, where the compiler's own choice of 46 held five: 6001 tokens 55 -> 47 us.
+template <int D>
+constexpr int AP_PER_SM = D <= 128 ? 8 : 4;
 
 struct AppendArgs {
     const float *q, *k, *v;
@@ -48,7 +53,7 @@ struct AppendArgs {
 
 // A warp holds a head as float4s: lane l elements 4l .. 4l+3 (+ 128 for d = 256).
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(AP_WARPS * 32) kv_append_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(AP_WARPS * 32, AP_PER_SM<D>) kv_append_kernel(const AppendArgs p) {
     constexpr int NV = (D + 127) / 128;        // float4s of a lane
     constexpr int LANES = D >= 128 ? 32 : D / 4;
     __shared__ float2 turn[D / 2];             // cos, sin

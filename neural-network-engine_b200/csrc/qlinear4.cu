@@ -44,56 +44,78 @@ __host__ __device__ inline size_t padded_groups(size_t chunks, int group) {
 }
 
 // ---- quantize ---------------------------------------------------------------------------------------------
-// A thread takes eight consecutive columns, a warp 256; a group is 4, 8 or 16 lanes, whose maximum is found by
-// shuffles, so a matrix is read once.  HBM bound: 4 bytes in and half a byte out per weight.
-__device__ __forceinline__ int code4(float v, float inv) {
-    const float t = __fmul_rn(v, inv);
-    if (!(t == t)) return 0;  // NaN
-    const float r = roundf(t);  // halves away from zero
-    return (int)fminf(fmaxf(r, -8.0f), 7.0f);
+// A warp takes 512 columns of a row, four runs of 128 with four consecutive columns a lane; a group is 8, 16 or 32 lanes,
+// whose maximum is found by shuffles, so a matrix is read once, 64 bytes a lane on their way.  HBM bound: 4 bytes in and half a
+// byte out per weight.
+//
+// round_half_away(t): |t| + 1/2 and the integer below it, both additions rounding towards zero, which crosses no integer
+// (0.49999997 + 0.5 rounded to nearest would be 1).  t is at most 7 but for its rounding, or, under a scale that has underflowed,
+// anything: the clamp comes first, to the same effect.
+__device__ __forceinline__ uint32_t code4(float v, float inv) {
+    float t = __fmul_rn(v, inv);
+    t = t == t ? fminf(fmaxf(t, -8.0f), 7.0f) : 0.0f;  // NaN: 0
+    const uint32_t magnitude = __float_as_uint(__fadd_rz(__fadd_rz(fabsf(t), 0.5f), 8388608.0f));  // the integer in the low bits
+    const uint32_t sign = (uint32_t)((int32_t)__float_as_uint(t) >> 31);
+    return ((magnitude ^ sign) - sign) & 15u;
 }
 
-template <bool VEC>
+template <bool VEC, int GROUP>
 __global__ void __launch_bounds__(256)
-quantize_rows4_kernel(const float *__restrict__ w, size_t rows, size_t cols, int group, uint8_t *__restrict__ q,
-                      float *__restrict__ scales) {
+quantize_rows4_kernel(const float *__restrict__ w, size_t rows, size_t cols, uint8_t *__restrict__ q, float *__restrict__ scales) {
+    constexpr int RUNS = 4, WIDE = RUNS * 128;
+    constexpr int width = GROUP / 4, per_run = 32 / width;  // lanes of a group, groups of a run
     const int lane = threadIdx.x & 31;
-    const size_t segs = (cols + 255) / 256, bytes = (cols + 1) / 2, groups = (cols + group - 1) / group;
-    const size_t total = rows * segs, step = (size_t)gridDim.x * 8;
-    const int width = group / 8;  // lanes of a group
-    for (size_t it = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < total; it += step) {
-        const size_t r = it / segs, c = (it - r * segs) * 256 + lane * 8;
-        const float *p = w + r * cols + c;
-        float v[8];
-        if (VEC) {  // cols % 8 == 0: a lane's columns are all there or all behind the row
+    const size_t segs = (cols + WIDE - 1) / WIDE, bytes = (cols + 1) / 2, groups = (cols + GROUP - 1) / GROUP;
+    const size_t step = (size_t)gridDim.x * 8, step_r = step / segs, step_s = step - step_r * segs;
+    const size_t first = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    size_t r = first / segs, seg = first - r * segs;
+    while (r < rows) {
+        float v[RUNS][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 f = c < cols ? __ldcs(reinterpret_cast<const float4 *>(p) + h) : make_float4(0, 0, 0, 0);
-                v[4 * h] = f.x, v[4 * h + 1] = f.y, v[4 * h + 2] = f.z, v[4 * h + 3] = f.w;
+        for (int k = 0; k < RUNS; ++k) {
+            const size_t c = seg * WIDE + k * 128 + lane * 4;
+            const float *p = w + r * cols + c;
+            if (VEC) {  // cols % 4 == 0: a lane's columns are all there or all behind the row
+                const float4 f = c < cols ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(0, 0, 0, 0);
+                v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[k][i] = c + i < cols ? p[i] : 0.0f;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? p[i] : 0.0f;
         }
+        // The 4 to 16 groups of the warp's columns, a lane each for the two divisions: in every lane they were half of
+        // the kernel's instructions.
         float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));  // NaN is passed over
-        for (int o = 1; o < width; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float scale = top > 0.0f ? __fdiv_rn(top, 7.0f) : 1.0f;
-        const float inv = __fdiv_rn(1.0f, scale);
-        uint32_t word = 0;
+        for (int k = 0; k < RUNS; ++k) {
+            float t = fmaxf(fmaxf(fabsf(v[k][0]), fabsf(v[k][1])), fmaxf(fabsf(v[k][2]), fabsf(v[k][3])));  // NaN is passed over
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= (uint32_t)(code4(v[i], inv) & 15) << (4 * i);
-        if (c >= cols) continue;  // after the shuffles
-        if (lane % width == 0) scales[r * groups + c / group] = scale;
-        uint8_t *o = q + r * bytes + c / 2;
-        if (VEC) {
-            *reinterpret_cast<uint32_t *>(o) = word;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + 2 * i < cols) o[i] = (uint8_t)(word >> (8 * i));  // codes behind the row are 0
+            for (int o = 1; o < width; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            t = __shfl_sync(0xffffffffu, t, (lane % per_run) * width);
+            if (lane / per_run == k) top = t;
         }
+        const float scale_of = top > 0.0f ? __fdiv_rn(top, 7.0f) : 1.0f;
+        const float inv_of = __fdiv_rn(1.0f, scale_of);
+#pragma unroll
+        for (int k = 0; k < RUNS; ++k) {
+            const size_t c = seg * WIDE + k * 128 + lane * 4;
+            const float scale = __shfl_sync(0xffffffffu, scale_of, k * per_run + lane / width);
+            const float inv = __shfl_sync(0xffffffffu, inv_of, k * per_run + lane / width);
+            uint32_t word = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word |= code4(v[k][i], inv) << (4 * i);
+            if (c >= cols) continue;  // after the shuffles
+            if (lane % width == 0) scales[r * groups + c / GROUP] = scale;
+            uint8_t *o = q + r * bytes + c / 2;
+            if (VEC) {
+                *reinterpret_cast<uint16_t *>(o) = (uint16_t)word;
+            } else {
+                o[0] = (uint8_t)word;  // codes behind the row are 0
+                if (c + 2 < cols) o[1] = (uint8_t)(word >> 8);
+            }
+        }
+        seg += step_s, r += step_r;
+        if (seg >= segs) seg -= segs, ++r;
     }
 }
 
@@ -628,12 +650,12 @@ unsigned grid_of(const nne_ctx *ctx, size_t items, size_t per_block) {
 
 int launch_quantize4(nne_ctx *ctx, const float *w, size_t rows, size_t cols, int group, uint8_t *q, float *scales, cudaStream_t s) {
     if (rows == 0 || cols == 0) return NNE_OK;
-    const unsigned grid = grid_of(ctx, rows * ((cols + 255) / 256), 8);
-    const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-    if (vec)
-        quantize_rows4_kernel<true><<<grid, 256, 0, s>>>(w, rows, cols, group, q, scales);
-    else
-        quantize_rows4_kernel<false><<<grid, 256, 0, s>>>(w, rows, cols, group, q, scales);
+    const unsigned grid = grid_of(ctx, rows * ((cols + 511) / 512), 8);
+    const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 1) == 0;
+    auto kernel = group == 32   ? (vec ? quantize_rows4_kernel<true, 32> : quantize_rows4_kernel<false, 32>)
+                  : group == 64 ? (vec ? quantize_rows4_kernel<true, 64> : quantize_rows4_kernel<false, 64>)
+                                : (vec ? quantize_rows4_kernel<true, 128> : quantize_rows4_kernel<false, 128>);
+    kernel<<<grid, 256, 0, s>>>(w, rows, cols, q, scales);
     NNE_LAUNCH_CHECK();
     return NNE_OK;
 }
