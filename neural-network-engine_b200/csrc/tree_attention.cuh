@@ -107,6 +107,21 @@ __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// The same from an accumulator of 0, which is no register: the first MMA of a chain.
+template <typename T>
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_first<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+template <>
+__device__ __forceinline__ void mma_first<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 // 2^x; below 2^-126: 0.
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -406,12 +421,6 @@ tree_attention_kernel(const TreeArgs p) {
         if (wn * 8 * NT < nrows) {  // a warp without rows only helps to load
             // S^T: the small parts of q in one accumulator, the large one in another
             float s[KM][NT][4], s2[KM][NT][4];
-#pragma unroll
-            for (int k = 0; k < KM; ++k)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[k][n][e] = s2[k][n][e] = 0.0f;
             const uint32_t ka = kt + (wk * KM * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
             const uint2 *qf = qfrag + (wn * NT) * (D / 16) * 32 + lane;
 #pragma unroll
@@ -426,8 +435,9 @@ tree_attention_kernel(const TreeArgs p) {
                         const uint2 w = qf[((q * (ROWS / 8) + n) * (D / 16) + step) * 32];
 #pragma unroll
                         for (int k = 0; k < KM; ++k) {
-                            if (q == 0) mma_16x8x16<T>(s[k][n], a[k], w.x, w.y);
-                            else mma_16x8x16<T>(s2[k][n], a[k], w.x, w.y);
+                            float(&acc)[4] = q == 0 ? s[k][n] : s2[k][n];
+                            if (step == 0 && q < 2) mma_first<T>(acc, a[k], w.x, w.y);
+                            else mma_16x8x16<T>(acc, a[k], w.x, w.y);
                         }
                     }
             }
@@ -508,10 +518,6 @@ tree_attention_kernel(const TreeArgs p) {
             for (int i = 0; i < D / 16; i += W) {
                 float add[W][NT][4];
 #pragma unroll
-                for (int w = 0; w < W; ++w)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) add[w][n][0] = add[w][n][1] = add[w][n][2] = add[w][n][3] = 0.0f;
-#pragma unroll
                 for (int k = 0; k < KM; ++k) {
                     uint32_t a[W][4];
 #pragma unroll
@@ -521,7 +527,10 @@ tree_attention_kernel(const TreeArgs p) {
 #pragma unroll
                         for (int w = 0; w < W; ++w)
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[w][n], a[w], pf[k][n][q][0], pf[k][n][q][1]);
+                            for (int n = 0; n < NT; ++n) {
+                                if (k == 0 && q == 0) mma_first<T>(add[w][n], a[w], pf[k][n][q][0], pf[k][n][q][1]);
+                                else mma_16x8x16<T>(add[w][n], a[w], pf[k][n][q][0], pf[k][n][q][1]);
+                            }
                 }
 #pragma unroll
                 for (int w = 0; w < W; ++w)
@@ -715,12 +724,6 @@ __global__ void __launch_bounds__(DecodeShape<T, D, NT>::THREADS, DecodeShape<T,
         // the one before it in its chain
         constexpr int CH = NT == 1 ? 2 : 1;
         float s[NT][4], sp[CH][PARTS][NT][4];
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) sp[c][q][n][0] = sp[c][q][n][1] = sp[c][q][n][2] = sp[c][q][n][3] = 0.0f;
         const uint32_t ka = kt + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (lane >> 4) * 16;
 #pragma unroll
         for (int step = 0; step < D / 16; ++step) {
@@ -734,7 +737,8 @@ __global__ void __launch_bounds__(DecodeShape<T, D, NT>::THREADS, DecodeShape<T,
                     uint2 w;
                     if constexpr (S::Q_REGS) w = qr[at];
                     else w = qfrag[at * 32 + lane];
-                    mma_16x8x16<T>(sp[step % CH][q][n], a, w.x, w.y);
+                    if (step < CH) mma_first<T>(sp[step % CH][q][n], a, w.x, w.y);
+                    else mma_16x8x16<T>(sp[step % CH][q][n], a, w.x, w.y);
                 }
         }
 #pragma unroll
@@ -800,15 +804,16 @@ __global__ void __launch_bounds__(DecodeShape<T, D, NT>::THREADS, DecodeShape<T,
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 ldsm_x4_trans(a[w], va + (i + w) * 32);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) add[w][n][0] = add[w][n][1] = add[w][n][2] = add[w][n][3] = 0.0f;
             }
 #pragma unroll
             for (int q = 0; q < PARTS; ++q)
 #pragma unroll
                 for (int w = 0; w < W; ++w)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16x8x16<T>(add[w][n], a[w], pf[n][q][0], pf[n][q][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        if (q == 0) mma_first<T>(add[w][n], a[w], pf[n][q][0], pf[n][q][1]);
+                        else mma_16x8x16<T>(add[w][n], a[w], pf[n][q][0], pf[n][q][1]);
+                    }
 #pragma unroll
             for (int w = 0; w < W; ++w)
 #pragma unroll
@@ -1043,6 +1048,9 @@ int launch_tree_d(nne_ctx *ctx, const TreeArgs &a, int sequences, long long max_
     if (rows <= 8) return launch_decode<T, D, 1>(ctx, a, sequences, rows, max_keys, s);
     if constexpr (D <= 128) {
         if (rows <= 16) return launch_decode<T, D, 2>(ctx, a, sequences, rows, max_keys, s);
+        // 8 rows a warp: twice the warps to hide each other's latency (8 trees of 8, bf16: 62 -> 58 us); 16 rows a warp: half
+        // the shared-memory traffic a product (64 nodes, f16: 92 -> 86 us)
+        if (rows <= 32) return launch_tree_shape<T, D, 1, 4, 2>(ctx, a, sequences, rows, max_keys, s);
         return launch_tree_shape<T, D, 2, 2, 2>(ctx, a, sequences, rows, max_keys, s);
     } else {
         if (rows <= 16) return launch_tree_shape<T, D, 1, 2, 2>(ctx, a, sequences, rows, max_keys, s);
