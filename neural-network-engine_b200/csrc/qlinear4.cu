@@ -251,11 +251,15 @@ template <int NT>
 struct Q4Shape {
     static constexpr int COLS = 4 * NT;                  // activation rows of a CTA
     static constexpr int CHUNK_BYTES = 4 * NT * 256;     // fragments of 64 columns
-    // Row tiles (one a warp) of a CTA.  With 32 activation rows a CTA has an SM to itself, so that a buffer of
-    // fragments serves twice the weight rows.
-    static constexpr int WARPS = NT >= 8 ? 16 : 8;
+    // Warps of a CTA, row tiles of a warp, CTAs of an SM.  With 32 activation rows the fragments' way out of shared memory
+    // would be the limit (79 % of it busy at one tile a warp), so each serves two tiles, and a CTA has an SM to itself: 48 rows of
+    // 4096 -> 11008 79 -> 66 us.
+    static constexpr int WARPS = 8;
+    static constexpr int TPW = NT >= 8 ? 2 : 1;
+    static constexpr int PER_SM = NT >= 8 ? 1 : 2;
+    static constexpr int TILES = WARPS * TPW;
     template <int GROUP>
-    __host__ __device__ static constexpr int slot() {  // bytes of a ring slot: codes, scales
+    __host__ __device__ static constexpr int slot() {  // bytes of a tile in a ring slot: codes, scales
         return Q4_CHUNK * Q4_ROWS / 2 + (GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP) * 64;
     }
 };
@@ -350,16 +354,16 @@ __global__ void __launch_bounds__(256) q4_prepare_kernel(const Q4Args p, uint8_t
 }
 
 template <int GROUP, int NT, bool READY>
-__global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WARPS) q4_forward_kernel(const Q4Args p) {
+__global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) q4_forward_kernel(const Q4Args p) {
     using S = Q4Shape<NT>;
-    constexpr int WARPS = S::WARPS, ROWS = WARPS * Q4_ROWS, D = Q4_DEPTH;
+    constexpr int WARPS = S::WARPS, TPW = S::TPW, ROWS = S::TILES * Q4_ROWS, D = Q4_DEPTH;
     constexpr int GPC = GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP;   // groups of a chunk
     constexpr int CPG = GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1;   // chunks of a group
     constexpr int SLOT = S::template slot<GROUP>();
     extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned split = gridDim.x, rank = blockIdx.x;
-    const unsigned tile = blockIdx.y * WARPS + warp;
+    const unsigned tile = blockIdx.y * S::TILES + warp * TPW;  // the warp's first
     const size_t row0 = (size_t)blockIdx.z * S::COLS;  // first activation row
     const unsigned cols = (unsigned)(p.m - row0 < (size_t)S::COLS ? p.m - row0 : S::COLS);
     const unsigned c_begin = rank * p.span < p.chunks ? rank * p.span : p.chunks;
@@ -369,16 +373,23 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WAR
     // The warp's ring of weight tiles: slot j holds chunk c with (c - c_begin) % D == j, a lane's 16 bytes copied by
     // that lane, and behind the codes the scales of the chunk's groups.  One copy group a chunk, also where a chunk has
     // no copy to make, so that "all but the last D - 2 groups" is always chunk c.
-    uint8_t *ring = smem + warp * (D * SLOT);
-    uint8_t *xbuf = smem + WARPS * D * SLOT;
+    uint8_t *ring = smem + warp * (D * TPW * SLOT);
+    uint8_t *xbuf = smem + S::TILES * D * SLOT;
     const uint32_t ring_at = smem_u32(ring) + lane * 16;
     const uint4 *wp = p.words + ((size_t)(mine ? tile : 0) * p.chunks + c_begin) * 32 + lane;
     const float2 *sp = p.scales + ((size_t)(mine ? tile : 0) * p.pgroups + q4_group<GROUP>(c_begin, 0)) * 8 + lane * 2;
+    const size_t w_next = tile + 1 < p.tiles ? (size_t)p.chunks * 32 : 0, s_next = tile + 1 < p.tiles ? (size_t)p.pgroups * 8 : 0;
     // chunk c_begin + at + j: `at` a multiple of D, so that the slot and the offsets are known when compiled
     auto fetch = [&](unsigned at, int j, bool there) {
         if (there) {
-            cp_async_16(ring_at + (j % D) * SLOT, wp + (size_t)at * 32 + j * 32);
-            if (lane < GPC * 4) cp_async_16(ring_at + (j % D) * SLOT + 512, sp + (size_t)(at / CPG * GPC) * 8 + (j / CPG) * GPC * 8);
+#pragma unroll
+            for (int u = 0; u < TPW; ++u) {
+                // a tile behind the last reads the last's: its sums are not stored
+                const size_t w_off = u == 0 ? 0 : w_next, s_off = u == 0 ? 0 : s_next;
+                const uint32_t dst = ring_at + ((j % D) * TPW + u) * SLOT;
+                cp_async_16(dst, wp + w_off + (size_t)at * 32 + j * 32);
+                if (lane < GPC * 4) cp_async_16(dst + 512, sp + s_off + (size_t)(at / CPG * GPC) * 8 + (j / CPG) * GPC * 8);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -389,9 +400,11 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WAR
     grid_dependency_wait();
     grid_launch_dependents();
 
-    float sum[NT][2], part[NT][4];
+    float sum[TPW][NT][2], part[TPW][NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = 0.0f;
+    for (int u = 0; u < TPW; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sum[u][t][0] = sum[u][t][1] = 0.0f;
 
     // Prepared activations of the chunks from s0 (counted in the share) on: 16-byte copies into buffer `buf`, part of
     // the copy group that is committed next.
@@ -455,20 +468,25 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WAR
             asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
             __syncwarp();  // the slot's scales are there for every lane, and the slot before has been read by every lane
             fetch(at, j + D - 1, more);
-            const uint8_t *slot = ring + j * SLOT;
-            const uint4 w4 = reinterpret_cast<const uint4 *>(slot)[lane];
-            const float2 *sc = reinterpret_cast<const float2 *>(slot + 512) + (lane >> 2);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            const uint8_t *slot = ring + j * TPW * SLOT;
+            uint32_t w[TPW][4];
+#pragma unroll
+            for (int u = 0; u < TPW; ++u) {
+                const uint4 w4 = reinterpret_cast<const uint4 *>(slot + u * SLOT)[lane];
+                w[u][0] = w4.x, w[u][1] = w4.y, w[u][2] = w4.z, w[u][3] = w4.w;
+            }
             const uint4 *fc = reinterpret_cast<const uint4 *>(here + (at - s0) * S::CHUNK_BYTES) + j * (S::CHUNK_BYTES / 16) + lane;
             const float4 *ic = info + (at - s0) / CPG * GPC * S::COLS + (lane & 3);
 #pragma unroll
             for (int pair = 0; pair < 2; ++pair) {
-                uint32_t a[2][4];
+                uint32_t a[TPW][2][4];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const uint32_t lo = w[2 * pair + q], up = lo >> 8;
-                    a[q][0] = lo & 0x000f000fu, a[q][1] = lo & 0x00f000f0u, a[q][2] = up & 0x000f000fu, a[q][3] = up & 0x00f000f0u;
-                }
+                for (int u = 0; u < TPW; ++u)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t lo = w[u][2 * pair + q], up = lo >> 8;
+                        a[u][q][0] = lo & 0x000f000fu, a[u][q][1] = lo & 0x00f000f0u, a[u][q][2] = up & 0x000f000fu, a[u][q][3] = up & 0x00f000f0u;
+                    }
                 const bool first = pair == 0 ? (CPG == 1 || j % CPG == 0) : GPC == 2;
                 const bool last = pair == 0 ? GPC == 2 : (CPG == 1 || j % CPG == CPG - 1 || end);
                 const int grp = CPG > 1 ? j / CPG : j * GPC + (GPC == 2 ? pair : 0);
@@ -477,18 +495,28 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WAR
                     const uint4 b = fc[(pair * NT + t) * 32];
                     if (first) {
                         const float2 i0 = *reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4);
-                        part[t][0] = i0.x, part[t][1] = i0.y, part[t][2] = 16.0f * i0.x, part[t][3] = 16.0f * i0.y;
+#pragma unroll
+                        for (int u = 0; u < TPW; ++u)
+                            part[u][t][0] = i0.x, part[u][t][1] = i0.y, part[u][t][2] = 16.0f * i0.x, part[u][t][3] = 16.0f * i0.y;
                     }
-                    mma_f16(part[t], a[0], b.x, b.y);
-                    mma_f16(part[t], a[1], b.z, b.w);
+#pragma unroll
+                    for (int u = 0; u < TPW; ++u) mma_f16(part[u][t], a[u][0], b.x, b.y);
+#pragma unroll
+                    for (int u = 0; u < TPW; ++u) mma_f16(part[u][t], a[u][1], b.z, b.w);
                 }
                 if (last) {
-                    const float2 s2 = sc[GPC == 2 ? pair * 8 : 0];
+                    float2 s2[TPW];
+#pragma unroll
+                    for (int u = 0; u < TPW; ++u)
+                        s2[u] = reinterpret_cast<const float2 *>(slot + u * SLOT + 512)[(lane >> 2) + (GPC == 2 ? pair * 8 : 0)];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         const float2 f = *(reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4) + 1);
-                        sum[t][0] = fmaf(s2.x * f.x, fmaf(part[t][0], 4096.0f, part[t][1]), sum[t][0]);
-                        sum[t][1] = fmaf(s2.y * f.y, fmaf(part[t][2], 4096.0f, part[t][3]), sum[t][1]);
+#pragma unroll
+                        for (int u = 0; u < TPW; ++u) {
+                            sum[u][t][0] = fmaf(s2[u].x * f.x, fmaf(part[u][t][0], 4096.0f, part[u][t][1]), sum[u][t][0]);
+                            sum[u][t][1] = fmaf(s2[u].y * f.y, fmaf(part[u][t][2], 4096.0f, part[u][t][3]), sum[u][t][1]);
+                        }
                     }
                 }
             }
@@ -510,10 +538,13 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, 16 / Q4Shape<NT>::WAR
     float *mysum = reinterpret_cast<float *>(smem);
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        mysum[(warp * 16 + (lane >> 2)) * S::COLS + t * 4 + (lane & 3)] = sum[t][0];
-        mysum[(warp * 16 + (lane >> 2) + 8) * S::COLS + t * 4 + (lane & 3)] = sum[t][1];
-    }
+    for (int u = 0; u < TPW; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = (warp * TPW + u) * Q4_ROWS + (lane >> 2);
+            mysum[r * S::COLS + t * 4 + (lane & 3)] = sum[u][t][0];
+            mysum[(r + 8) * S::COLS + t * 4 + (lane & 3)] = sum[u][t][1];
+        }
     if (split > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else {
@@ -546,22 +577,26 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
     using S = Q4Shape<NT>;
     constexpr bool READY = NT > 1;
     const nne_ctx *ctx = ql->ctx;
-    const size_t blocks_n = (ql->tiles + S::WARPS - 1) / S::WARPS;
+    const size_t blocks_n = (ql->tiles + S::TILES - 1) / S::TILES;
     const size_t blocks_m = (m + S::COLS - 1) / S::COLS;
     if (blocks_n > 65535 || blocks_m > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "layer or batch too large for one launch");
-    // Split the columns over as many CTAs as the GPU holds at once - one more and a second round would run nearly
-    // empty (28672 -> 8192, one row, group 64, in 320 CTAs: 54 us, in 256: 31) - as long as a share keeps eight chunks of 64.
-    const size_t slots = (size_t)ctx->sm_count * (16 / S::WARPS), have = blocks_n * blocks_m;
-    size_t split = slots / have;
-    split = split < 1 ? 1 : (split > Q4_MAX_SPLIT ? Q4_MAX_SPLIT : split);
-    while (split > 1 && ql->chunks < split * 8) --split;
+    // Split the columns over the CTAs of a cluster: a CTA's time is its chunks and, in their measure, about ten for starting,
+    // activations and the join, and CTAs run in rounds of what the GPU holds (28672 -> 8192, one row, in 320 CTAs: 54
+    // us, in 256: 31).  A share keeps eight chunks of 64.
+    const size_t slots = (size_t)ctx->sm_count * S::PER_SM, have = blocks_n * blocks_m;
+    size_t split = 1;
+    double least = 1e300;
+    for (size_t c = 1; c <= Q4_MAX_SPLIT && (c == 1 || ql->chunks >= c * 8); ++c) {
+        const double cost = (double)((have * c + slots - 1) / slots) * ((double)ql->chunks / (double)c + 10.0);
+        if (cost < least * 0.98) split = c, least = cost;
+    }
     // shares in whole pairs of chunks, so that a group of 128 columns never lies in two
     size_t span = (ql->chunks + split - 1) / split;
     span = (span + 1) & ~(size_t)1;
     split = (ql->chunks + span - 1) / span;
     // Activations in shared memory beside the weight rings, in stages of whole ring rounds: two buffers for prepared
     // ones (the next stage is copied in during this one), one for those the CTA prepares.
-    const size_t ring = (size_t)S::WARPS * Q4_DEPTH * S::template slot<GROUP>();
+    const size_t ring = (size_t)S::TILES * Q4_DEPTH * S::template slot<GROUP>();
     auto xbytes = [](size_t chunks) { return chunks * S::CHUNK_BYTES + q4_groups<GROUP>((unsigned)chunks) * S::COLS * sizeof(float4); };
     size_t stage = READY ? Q4_DEPTH : 7 * Q4_DEPTH;
     if (stage >= span) stage = span;
@@ -582,7 +617,7 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
     a.stage = (unsigned)stage;
     a.vec = ql->k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     size_t bytes = ring + xbytes(stage) * (READY && stage < span ? 2 : 1);
-    const size_t sums = (size_t)S::WARPS * Q4_ROWS * S::COLS * sizeof(float);
+    const size_t sums = (size_t)S::TILES * Q4_ROWS * S::COLS * sizeof(float);
     if (bytes < sums) bytes = sums;
     NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT, READY>, bytes));
 
