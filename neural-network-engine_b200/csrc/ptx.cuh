@@ -206,6 +206,14 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// All threads of all CTAs of the cluster meet; what they wrote before is seen by all afterwards.  Not the `.aligned` form, which
+// a warp that has not come back together must not execute.  A value that a thread has loaded from another CTA's shared memory has to
+// have been used before the last meeting: a load that nothing waits for can still be on its way when the CTA it goes to leaves.
+__device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // Host: encodes a 2-D tiled tensor map (row-major [outer, inner], box [box_outer, box_inner]).
 int tma_make_map_2d(CUtensorMap *map, CUtensorMapDataType dt, size_t elem_bytes, const void *base,
                     size_t inner, size_t outer, uint32_t box_inner, uint32_t box_outer,

@@ -216,7 +216,7 @@ dequantize4_kernel(const uint4 *__restrict__ words, const float2 *__restrict__ s
 //  At a group's end 4096 * (hi sum) + (lo sum) rounds once and joins the row's f32 sum with scale * 2^-e.  The error is
 //  that of f32 (x off by 2^-23 of its group's largest); one f16 for x would give 2^-11.
 //
-// A CTA takes 128 or 256 rows (a tile a warp) and a share of the columns; the CTAs of a cluster take the shares of one
+// A CTA takes 128 or 256 rows (one or two tiles a warp) and a share of the columns; the CTAs of a cluster take the shares of one
 // row block and add their sums up through each other's shared memory in rank order, so results do not change from
 // run to run.  Each warp streams its weights through a ring of its own, filled by asynchronous copies seven tiles ahead
 // that start before the wait for the kernel that makes x (a layer never changes); no other warp is waited for.  (The same
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
             mysum[(r + 8) * S::COLS + t * 4 + (lane & 3)] = sum[u][t][1];
         }
     if (split > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_meet();
     } else {
         __syncthreads();
     }
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
         p.y[(row0 + c) * p.ldy + out0 + r] = v;
     }
     if (split > 1)  // nobody leaves while a peer may still read its shared memory
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_meet();
 }
 
 template <int GROUP, int NT>

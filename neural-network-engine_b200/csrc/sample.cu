@@ -68,9 +68,6 @@ struct Shared {
     unsigned kept;
 };
 
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ unsigned long long ld_cluster_u64(const void *p, unsigned rank) {
     uint32_t peer;
     unsigned long long v;
@@ -86,6 +83,15 @@ __device__ __forceinline__ unsigned ld_cluster_u32(const void *p, unsigned rank)
     return v;
 }
 
+// One thread a warp looks, all have the value - and have waited for it - when this returns.
+__device__ __forceinline__ unsigned ask_cluster_u32(const void *p, unsigned rank) {
+    const unsigned v = (threadIdx.x & 31) == 0 ? ld_cluster_u32(p, rank) : 0;
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+__device__ __forceinline__ unsigned long long ask_cluster_u64(const void *p, unsigned rank) {
+    const unsigned long long v = (threadIdx.x & 31) == 0 ? ld_cluster_u64(p, rank) : 0;
+    return __shfl_sync(0xffffffffu, v, 0);
+}
 __device__ __forceinline__ unsigned add_cluster_u32(const void *p, unsigned rank, unsigned v) {
     uint32_t peer;
     unsigned old;
@@ -245,7 +251,8 @@ struct Row {
             const unsigned long long u = __shfl_up_sync(0xffffffffu, upto, o);
             if ((int)(threadIdx.x & 31) >= o) upto += u;
         }
-        const unsigned owner = __ffs(__ballot_sync(0xffffffffu, upto > want)) - 1;
+        const unsigned reached = __ballot_sync(0xffffffffu, upto > want) & ((1u << ranks) - 1);
+        const unsigned owner = reached ? __ffs(reached) - 1 : ranks - 1;  // (nothing to locate: the last, which finds no place)
         unsigned long long before = __shfl_sync(0xffffffffu, upto - part, (int)owner);
         if (owner == rank) {  // the warp whose part holds it, then all threads on that part, a few logits each
             int warp = 0;
@@ -260,12 +267,13 @@ struct Row {
             unsigned long long run = before + v[0] - own;
             if (run <= want && run + own > want) {  // one thread
                 unsigned i = from;
-                while ((run += f(i, l[i])) <= want) ++i;
+                for (; i + 1 < to; ++i)
+                    if ((run += f(i, l[i])) > want) break;
                 s->found = i;
             }
         }
         cluster_meet();
-        return ld_cluster_u32(&s->found, owner);
+        return ask_cluster_u32(&s->found, owner);
     }
 
     // The draw itself: the first index at which the mass of what `kept` and min_p leave exceeds u * that mass.
@@ -420,15 +428,17 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
     const float inv = __fdiv_rn(SM_PER_T, r.temperature);
     if (!(inv < 1e30f) || isinf(r.top)) return -2;  // distances need numbers to be measured in
     const bool by_mass = set.top_p < 1.0f;
-    auto distance = [&](float x) { return (r.top - x) * inv; };  // in sixteenths of T; never falls as x falls
+    // in sixteenths of T; never falls as x falls.  Products and differences that are rounded one by one: every pass has to find a
+    // token in the same bucket
+    auto distance = [&](float x) { return __fmul_rn(__fsub_rn(r.top, x), inv); };
     // Buckets: of one sixteenth up to 12 T, of a quarter up to 28 T, where a mass is less than a unit and counts as none; or 256
     // in the place of one of those, [lo, hi).
     constexpr float END = 4.0f * SM_BUCKETS - 3.0f * SM_FINE;
     float lo = 0.0f, hi = END, per = 1.0f;
     bool whole = true;
     auto bucket = [&](float d) {  // of a distance in [lo, hi)
-        const float t = (d - lo) * per;
-        return min(whole && t >= (float)SM_FINE ? SM_FINE + (int)((t - (float)SM_FINE) * 0.25f) : (int)t, SM_BUCKETS - 1);
+        const float t = __fmul_rn(__fsub_rn(d, lo), per);
+        return min(whole && t >= (float)SM_FINE ? SM_FINE + (int)__fmul_rn(__fsub_rn(t, (float)SM_FINE), 0.25f) : (int)t, SM_BUCKETS - 1);
     };
     auto first = [&](auto &&reached) {  // of the buckets; SM_BUCKETS: none
         int from = 0, to = SM_BUCKETS;
@@ -489,7 +499,7 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
             }
         });
         cluster_meet();
-        return ld_cluster_u32(&s->listed, 0);
+        return ask_cluster_u32(&s->listed, 0);
     };
     const float far = set.min_p > 0.0f ? -logf(set.min_p) * SM_PER_T + 1.0f : END;  // what is farther min_p leaves out
 
@@ -605,7 +615,7 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
                     }
                 }
                 cluster_meet();
-                const unsigned long long cut = ld_cluster_u64(&s->above, 0);
+                const unsigned long long cut = ask_cluster_u64(&s->above, 0);
                 edge = logit_of((uint32_t)(cut >> 32));
                 index = 0xffffffffu - (unsigned)cut;
                 cluster_meet();  // rank 0 goes on to use the word
@@ -731,7 +741,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     r.end = min(r.begin + r.warp_span, r.cta_end);
     for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
     for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.count[0][i] = sh.low[0][i] = sh.high[0][i] = 0;
-    if (threadIdx.x == 0) sh.listed = sh.kept = 0;
+    if (threadIdx.x == 0) sh.listed = sh.kept = sh.found = 0;
 
     // Settings now: their latency passes under the first pass.
     const float t = p.temperature ? p.temperature[row] : 1.0f, u = p.uniform[row];

@@ -146,9 +146,6 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t at, uint32_t rank) {
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer) : "memory");
     return v;
 }
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // Queries: scale * log2(e) * q, as parts of the cache's type in the MMA's operand order [part][8-row tile][step][lane].
 // f16: times a power of two that brings a row's largest to [2^13, 2^14), undone by qfac.  vis: what a row's node sees.
