@@ -62,7 +62,9 @@ struct Shared {
     unsigned found;
     int bucket;
     unsigned long long above;
-    unsigned count[2][SM_BUCKETS], low[2][SM_BUCKETS], high[2][SM_BUCKETS], all_count[SM_BUCKETS];
+    // Sets of levels 0 and 1; count's third is that of the threads' maxima.  Each its own: no meeting lies between the looks into
+    // one and the first atomics on the next.
+    unsigned count[3][SM_BUCKETS], low[2][SM_BUCKETS], high[2][SM_BUCKETS], all_count[SM_BUCKETS];
     unsigned long long list[SM_LIST];
     unsigned listed;
     unsigned kept;
@@ -134,7 +136,7 @@ struct Row {
     float top, temperature, scale;
 
     // A token's weight, and that in units of 2^-40 (the rest of a unit is dropped).  scale: log2(e) / T.
-    __device__ __forceinline__ float weight(float x) const { 
+    __device__ __forceinline__ float weight(float x) const {
         float w;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf(x - top, -3.402823466e38f) * scale));
         return x == top ? 1.0f : w;
@@ -739,8 +741,9 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
     r.cta_begin = min(r.rank * span, p.vocab), r.cta_end = min(r.cta_begin + span, p.vocab);
     r.begin = min(r.cta_begin + (threadIdx.x >> 5) * r.warp_span, r.cta_end);
     r.end = min(r.begin + r.warp_span, r.cta_end);
-    for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
-    for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.count[0][i] = sh.low[0][i] = sh.high[0][i] = 0;
+    for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) (&sh.mass[0][0])[i] = 0;
+    for (int i = threadIdx.x; i < 3 * SM_BUCKETS; i += SM_THREADS) (&sh.count[0][0])[i] = 0;
+    for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) (&sh.low[0][0])[i] = (&sh.high[0][0])[i] = 0;
     if (threadIdx.x == 0) sh.listed = sh.kept = sh.found = 0;
 
     // Settings now: their latency passes under the first pass.
@@ -779,7 +782,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(r, set, top);
         if (token == -2) {
             cluster_meet();  // the buckets have been read by everybody
-            for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) sh.mass[0][i] = 0;
+            for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) (&sh.mass[0][0])[i] = 0;
             token = draw_by_search(r, top_key, p.vocab, set);
         }
     }

@@ -110,6 +110,21 @@ def test_ties(nne, ctx, vocab):
     check(nne, ctx, logits, np.float32(0.9999), 0.5, k, p, 0.2)
 
 
+@pytest.mark.parametrize("vocab", [20000, 70000])
+def test_a_top_k_beyond_the_threads(nne, ctx, vocab):
+    """More places than a cluster has threads (2048 at this many rows), with and without top-p."""
+    rng = np.random.default_rng(6)
+    rows = 64
+    logits = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    logits[::2, : vocab // 2] -= 12.0                      # a cluster's parts that differ in their work
+    logits[1::4] = np.round(logits[1::4])
+    k = rng.choice([2049, 3000, 4100, 9001, vocab - 1], rows)
+    for _ in range(4):
+        u = rng.random(rows).astype(np.float32)
+        check(nne, ctx, logits, u, 1.0, k, rng.choice([0.9, 0.5, 0.1, 1.0], rows).astype(np.float32))
+        check(nne, ctx, logits, u, 0.7, k)
+
+
 @pytest.mark.parametrize("vocab", [64, 12345])
 def test_masked_and_special_logits(nne, ctx, vocab):
     rng = np.random.default_rng(3)
