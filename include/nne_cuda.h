@@ -314,7 +314,7 @@ NNE_API int nne_qlinear_plan_create_fused(nne_ctx *ctx, size_t count, const nne_
  * holds Inf or NaN gives NaN or Inf in every channel whose codes meet it; other rows are untouched.
  * Up to four rows are one launch; more are two, with a stream-ordered workspace of about 4 * m * k bytes.  Weights are read once for up to 32 rows, once more for each further 32.
  * The handle is immutable and forwards may run concurrently, as with nne_qlinear.  Limits: 2^22 rows,
- * 2^30 columns. */
+ * 2^30 columns, 2^18 activation rows a call. */
 NNE_API int nne_quantize_rows4_dev(nne_ctx *ctx, const float *w_dev, size_t rows, size_t cols, size_t group,
                                    uint8_t *q_dev, float *scales_dev, void *stream);
 NNE_API int nne_qlinear4_create_from_f32(nne_ctx *ctx, const float *w_host, const float *bias_host_or_null,
@@ -330,8 +330,9 @@ NNE_API int nne_qlinear4_create_from_i4_dev(nne_ctx *ctx, const uint8_t *q_dev, 
                                             const float *bias_dev_or_null, size_t n, size_t k, size_t group,
                                             void *stream, nne_qlinear4 **out);
 NNE_API int nne_qlinear4_destroy(nne_qlinear4 *ql);
-/* Codes and scales in the public layout; either pointer may be NULL. */
-NNE_API int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host);
+/* Codes and scales in the public layout, and the bias [n] (untouched where the layer has none); any pointer
+ * may be NULL. */
+NNE_API int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host, float *bias_host);
 /* The f32 weights [n, k] the layer stands for, q * scale (as QLinear::to_linear, src/nn/quantized.rs:200-209). */
 NNE_API int nne_qlinear4_dequantize(const nne_qlinear4 *ql, float *w_host);
 NNE_API int nne_qlinear4_info(const nne_qlinear4 *ql, size_t *n, size_t *k, size_t *group, int *has_bias);
@@ -415,13 +416,13 @@ NNE_API int nne_kv_append_dev(nne_kv_cache *cache, const nne_kv_append *args, vo
  * node j's key in place context[b] + j.  Node i sees node j where bit j of visible[row of i] is set - its ancestors
  * and itself, as a rule - or, visible NULL, where j <= i (a chain); bits of nodes that are not there mean nothing.
  *     out[row, h] = softmax(scale * q[row, h] . k) v      over what the node sees, head h / (q_heads / kv_heads)
- * A row that sees nothing is 0.  What a row does not see does not reach it, Inf and NaN included.  Keys
- * whose place the table does not name, or in a page outside the pool, are seen by nobody.  q and out are f32,
- * [row][q_heads][head_dim] with a stride in floats from row to row, and do not overlap.  The products are of f32 accuracy (q
+ * A row that sees nothing is 0.  What a row does not see does not reach it, Inf and NaN included; Inf or NaN in a
+ * key that it sees makes it NaN, in a value Inf or NaN.  Keys whose place the table does not name, or in a page
+ * outside the pool, are seen by nobody.  q and out are f32, [row][q_heads][head_dim] with a stride in floats from row to row, and do not overlap.  The products are of f32 accuracy (q
  * and the probabilities keep 22 bits or more).  max_nodes (at most 64) bounds the nodes of a sequence: rows
  * of a sequence beyond it are not written; longer chains go through in pieces of 64, appended piece by piece.
- * max_context only guides how far the work is split; contexts may be longer.  One launch without workspace, or, few rows
- * over long contexts, two with a stream-ordered workspace of at most a few megabytes; asynchronous on `stream`.  Results
+ * At most 65535 sequences a call.  max_context only guides how far the work is split; contexts may be longer.  One
+ * launch without workspace, or, few rows over long contexts, two with a stream-ordered workspace of some megabytes; asynchronous on `stream`.  Results
  * do not change from run to run. */
 typedef struct nne_tree_attention {
     const float *q;

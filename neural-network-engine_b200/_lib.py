@@ -90,7 +90,7 @@ SIGNATURES = {
     "nne_qlinear4_create_from_i4_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                                   C.c_size_t, C.c_size_t, C.c_void_p, c_void_pp]),
     "nne_qlinear4_destroy": (C.c_int, [C.c_void_p]),
-    "nne_qlinear4_download": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nne_qlinear4_download": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "nne_qlinear4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nne_qlinear4_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t),
                                     C.POINTER(C.c_int)]),

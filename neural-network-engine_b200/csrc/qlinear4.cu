@@ -579,7 +579,6 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
     const nne_ctx *ctx = ql->ctx;
     const size_t blocks_n = (ql->tiles + S::TILES - 1) / S::TILES;
     const size_t blocks_m = (m + S::COLS - 1) / S::COLS;
-    if (blocks_n > 65535 || blocks_m > 65535) return fail(NNE_ERR_INVALID_ARGUMENT, "layer or batch too large for one launch");
     // Split the columns over the CTAs of a cluster: a CTA's time is its chunks and, in their measure, about ten for starting,
     // activations and the join, and CTAs run in rounds of what the GPU holds (28672 -> 8192, one row, in 320 CTAs: 54
     // us, in 256: 31).  A share keeps eight chunks of 64.
@@ -695,6 +694,11 @@ int launch_quantize4(nne_ctx *ctx, const float *w, size_t rows, size_t cols, int
     return NNE_OK;
 }
 
+int check_f32(const float *p) {
+    if (reinterpret_cast<uintptr_t>(p) & 3) return fail(NNE_ERR_INVALID_ARGUMENT, "an f32 device pointer is not 4-byte aligned");
+    return NNE_OK;
+}
+
 int check_group(size_t group) {
     if (group != 32 && group != 64 && group != 128)
         return fail(NNE_ERR_INVALID_ARGUMENT, "group must be 32, 64 or 128 columns, got %zu", group);
@@ -763,6 +767,7 @@ int forward4(nne_qlinear4 *ql, const float *x, size_t m, size_t k, float *y, siz
     size_t t;
     if (__builtin_mul_overflow(m, ql->k, &t) || __builtin_mul_overflow(m, ldy, &t) || __builtin_mul_overflow(t, sizeof(float), &t))
         return fail(NNE_ERR_INVALID_ARGUMENT, "m*k or m*ldy overflows size_t");
+    if (m > ((size_t)1 << 18)) return fail(NNE_ERR_INVALID_ARGUMENT, "at most 2^18 activation rows a call, got %zu", m);
     if (m == 0 || ql->n == 0) return NNE_OK;
     if (!y || (ql->k && !x)) return fail(NNE_ERR_INVALID_ARGUMENT, "null activation or output pointer");
     if ((reinterpret_cast<uintptr_t>(x) & 3) || (reinterpret_cast<uintptr_t>(y) & 3))
@@ -820,6 +825,8 @@ int nne_quantize_rows4_dev(nne_ctx *ctx, const float *w_dev, size_t rows, size_t
         return fail(NNE_ERR_INVALID_ARGUMENT, "rows*cols overflows size_t");
     if (rows == 0 || cols == 0) return NNE_OK;
     if (!w_dev || !q_dev || !scales_dev) return fail(NNE_ERR_INVALID_ARGUMENT, "null device pointer");
+    NNE_TRY(check_f32(w_dev));
+    NNE_TRY(check_f32(scales_dev));
     return launch_quantize4(ctx, w_dev, rows, cols, (int)group, q_dev, scales_dev, (cudaStream_t)stream);
     NNE_GUARD_END
 }
@@ -831,6 +838,7 @@ int nne_qlinear4_create_from_f32_dev(nne_ctx *ctx, const float *w_dev, const flo
     *out = nullptr;
     NNE_TRY(use_ctx(ctx));
     if (n && k && !w_dev) return fail(NNE_ERR_INVALID_ARGUMENT, "null weight pointer");
+    NNE_TRY(check_f32(w_dev));
     nne_qlinear4 *ql = nullptr;
     NNE_TRY(alloc_layer4(ctx, n, k, group, bias_dev_or_null != nullptr, &ql));
     const int st = quantize_into4(ql, w_dev, bias_dev_or_null, cudaMemcpyDeviceToDevice, (cudaStream_t)stream);
@@ -878,6 +886,7 @@ int nne_qlinear4_create_from_i4_dev(nne_ctx *ctx, const uint8_t *q_dev, const fl
     *out = nullptr;
     NNE_TRY(use_ctx(ctx));
     if (n && k && (!q_dev || !scales_dev)) return fail(NNE_ERR_INVALID_ARGUMENT, "null codes or scales pointer");
+    NNE_TRY(check_f32(scales_dev));
     nne_qlinear4 *ql = nullptr;
     NNE_TRY(alloc_layer4(ctx, n, k, group, bias_dev_or_null != nullptr, &ql));
     const int st = fill_layer4(ql, q_dev, scales_dev, bias_dev_or_null, cudaMemcpyDeviceToDevice, (cudaStream_t)stream);
@@ -934,22 +943,23 @@ int nne_qlinear4_destroy(nne_qlinear4 *ql) {
     NNE_GUARD_END
 }
 
-int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host) {
+int nne_qlinear4_download(const nne_qlinear4 *ql, uint8_t *q_host, float *scales_host, float *bias_host) {
     NNE_GUARD_BEGIN
     if (!ql || !ql->ctx) return fail(NNE_ERR_INVALID_ARGUMENT, "null layer handle");
-    if (ql->n == 0 || ql->k == 0) return NNE_OK;
+    if (ql->n == 0) return NNE_OK;
     NNE_TRY(use_ctx(ql->ctx));
     std::lock_guard<std::mutex> lock(ql->ctx->mu);
     cudaStream_t s = ql->ctx->stream;
     const size_t qb = ql->n * ((ql->k + 1) / 2), sb = ql->n * ql->groups * sizeof(float);
     Scratch q(s), sc(s);
-    if (q_host) {
+    if (bias_host && ql->bias) NNE_CUDA_TRY(cudaMemcpyAsync(bias_host, ql->bias, ql->n * sizeof(float), cudaMemcpyDeviceToHost, s));
+    if (q_host && ql->k) {
         NNE_TRY(q.get(qb));
         unpack_codes_kernel<<<grid_of(ql->ctx, qb, 256), 256, 0, s>>>(ql->words, ql->n, ql->k, ql->chunks, (uint8_t *)q.p);
         NNE_LAUNCH_CHECK();
         NNE_CUDA_TRY(cudaMemcpyAsync(q_host, q.p, qb, cudaMemcpyDeviceToHost, s));
     }
-    if (scales_host) {
+    if (scales_host && ql->k) {
         NNE_TRY(sc.get(sb));
         unpack_scales_kernel<<<grid_of(ql->ctx, ql->n * ql->groups, 256), 256, 0, s>>>(
             ql->scales, ql->n, ql->groups, padded_groups(ql->chunks, ql->group), (float *)sc.p);

@@ -28,12 +28,12 @@ def quantize_rows4_device(ctx: CudaContext, w_ptr: int, rows: int, cols: int, gr
 
 class QLinear4:
     """4-bit linear layer; ``qweight`` (uint8 ``[out_features, (in_features + 1) // 2]``) and ``scales`` (f32
-    ``[out_features, ceil(in_features / group)]``) are host copies, fetched from the device when first asked for."""
+    ``[out_features, ceil(in_features / group)]``) and ``bias`` are host copies, fetched from the device when first asked
+    for."""
 
-    def __init__(self, handle, in_features: int, out_features: int, group: int, bias, ctx: CudaContext):
+    def __init__(self, handle, in_features: int, out_features: int, group: int, ctx: CudaContext):
         self._handle, self._ctx = handle, ctx
         self.in_features, self.out_features, self.group = int(in_features), int(out_features), int(group)
-        self.bias = bias
         self._host = None
         # bound once: a forward is one foreign call, without a look-up on its way
         self._forward, self._forward_strided = load().nne_qlinear4_forward_dev, load().nne_qlinear4_forward_dev_strided
@@ -50,7 +50,7 @@ class QLinear4:
             check(load().nne_qlinear4_create_from_f32(ctx.handle, _ptr(w), _ptr(b), n, k, group, C.byref(h)))
         except NneError as e:
             _raise_mapped(e)
-        return cls(h, k, n, group, b, ctx)
+        return cls(h, k, n, group, ctx)
 
     @classmethod
     def from_fields(cls, qweight, scales, bias, in_features: int, out_features: int, group: int,
@@ -70,20 +70,20 @@ class QLinear4:
             check(load().nne_qlinear4_create_from_i4(ctx.handle, _ptr(q), _ptr(s), _ptr(b), n, k, group, C.byref(h)))
         except NneError as e:
             _raise_mapped(e)
-        return cls(h, k, n, group, b, ctx)
+        return cls(h, k, n, group, ctx)
 
     @classmethod
     def from_packed_device(cls, ctx: CudaContext, q_ptr: int, scales_ptr: int, bias_ptr: int, n: int, k: int, group: int,
                            stream: int = 0) -> "QLinear4":
         """From codes and scales in the public layout that are on the device (``bias_ptr`` 0: none).  The buffers are
-        not kept; ``bias`` of the object stays None, the device layer has it."""
+        not kept."""
         h = C.c_void_p()
         try:
             check(load().nne_qlinear4_create_from_i4_dev(ctx.handle, q_ptr, scales_ptr, bias_ptr or None, n, k, group, stream,
                                                          C.byref(h)))
         except NneError as e:
             _raise_mapped(e)
-        return cls(h, k, n, group, None, ctx)
+        return cls(h, k, n, group, ctx)
 
     @classmethod
     def from_linear_device(cls, ctx: CudaContext, w_ptr: int, bias_ptr: int, n: int, k: int, group: int = 128,
@@ -94,7 +94,7 @@ class QLinear4:
             check(load().nne_qlinear4_create_from_f32_dev(ctx.handle, w_ptr, bias_ptr or None, n, k, group, stream, C.byref(h)))
         except NneError as e:
             _raise_mapped(e)
-        return cls(h, k, n, group, None, ctx)
+        return cls(h, k, n, group, ctx)
 
     # -- fields ----------------------------------------------------------------------------------
     def _live_handle(self):
@@ -107,10 +107,13 @@ class QLinear4:
             q = np.zeros((self.out_features, (self.in_features + 1) // 2), dtype=np.uint8)
             s = np.zeros((self.out_features, -(-self.in_features // self.group)), dtype=np.float32)
             try:
-                check(load().nne_qlinear4_download(self._live_handle(), _ptr(q), _ptr(s)))
+                has_bias = C.c_int()
+                check(load().nne_qlinear4_info(self._live_handle(), None, None, None, C.byref(has_bias)))
+                b = np.zeros(self.out_features, dtype=np.float32) if has_bias.value else None
+                check(load().nne_qlinear4_download(self._live_handle(), _ptr(q), _ptr(s), _ptr(b)))
             except NneError as e:
                 _raise_mapped(e)
-            self._host = (q, s)
+            self._host = (q, s, b)
         return self._host
 
     @property
@@ -120,6 +123,10 @@ class QLinear4:
     @property
     def scales(self) -> np.ndarray:
         return self._fields()[1]
+
+    @property
+    def bias(self) -> Optional[np.ndarray]:
+        return self._fields()[2]
 
     def to_linear(self) -> Linear:
         """The f32 layer this one stands for, q * scale."""

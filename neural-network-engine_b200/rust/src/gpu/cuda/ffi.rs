@@ -386,7 +386,12 @@ extern "C" {
         out: *mut *mut nne_qlinear4,
     ) -> c_int;
     pub fn nne_qlinear4_destroy(ql: *mut nne_qlinear4) -> c_int;
-    pub fn nne_qlinear4_download(ql: *const nne_qlinear4, q_host: *mut u8, scales_host: *mut f32) -> c_int;
+    pub fn nne_qlinear4_download(
+        ql: *const nne_qlinear4,
+        q_host: *mut u8,
+        scales_host: *mut f32,
+        bias_host: *mut f32,
+    ) -> c_int;
     pub fn nne_qlinear4_dequantize(ql: *const nne_qlinear4, w_host: *mut f32) -> c_int;
     pub fn nne_qlinear4_info(
         ql: *const nne_qlinear4,

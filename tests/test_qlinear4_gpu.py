@@ -195,6 +195,26 @@ def test_device_layer_and_empty_cases(nne, ctx):
     assert ql.memory_bytes() == 16 * 64 // 2 + 16 * 2 * 4 + 4 * 4 and ql.parameters() == []
 
 
+def test_layers_made_on_the_device_give_their_fields_back(nne, ctx):
+    import torch
+    n, k, group = 19, 77, 32
+    w, bias = oracle.normal(716, 0, (n, k), 0.0, 0.02), oracle.normal(716, 1, (n,))
+    wd, bd = torch.from_numpy(w).cuda(), torch.from_numpy(bias).cuda()
+    s = torch.cuda.current_stream().cuda_stream
+    codes, scales = quantize4_numpy(w, group)
+    a = nne.QLinear4.from_linear_device(ctx, wd.data_ptr(), bd.data_ptr(), n, k, group, s)
+    qd, sd = torch.from_numpy(pack4(codes)).cuda(), torch.from_numpy(scales).cuda()
+    b = nne.QLinear4.from_packed_device(ctx, qd.data_ptr(), sd.data_ptr(), bd.data_ptr(), n, k, group, s)
+    c = nne.QLinear4.from_packed_device(ctx, qd.data_ptr(), sd.data_ptr(), 0, n, k, group, s)
+    for x in (a, b, c):
+        assert np.array_equal(x.qweight, pack4(codes)) and np.array_equal(x.scales, scales)
+    assert np.array_equal(a.bias, bias) and np.array_equal(b.to_linear().bias, bias) and c.bias is None
+    with pytest.raises(nne.InvalidArgument):
+        nne.QLinear4.from_packed_device(ctx, qd.data_ptr(), sd.data_ptr() + 2, 0, n, k, group, s)
+    with pytest.raises(nne.InvalidArgument):
+        nne.quantize_rows4_device(ctx, wd.data_ptr() + 1, 1, 4, group, qd.data_ptr(), sd.data_ptr(), s)
+
+
 def test_refusals(nne, ctx):
     w = nne.Linear(np.ones((4, 64), np.float32))
     for group in (0, 16, 48, 256):
