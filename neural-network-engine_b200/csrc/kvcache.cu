@@ -338,8 +338,10 @@ int nne_kv_append_dev(nne_kv_cache *c, const nne_kv_append *a, void *stream) {
     if (a->k && (!a->page_table || !a->sequence || !a->index || a->table_stride == 0 || a->sequences < 0))
         return fail(NNE_ERR_INVALID_ARGUMENT, "storing keys needs page_table, table_stride, sequence and index");
     if (c->rope_dims && !a->position && !a->index) return fail(NNE_ERR_INVALID_ARGUMENT, "a rotation needs position or index");
-    if (!is_aligned(a->q, 4) || !is_aligned(a->k, 4) || !is_aligned(a->v, 4) || !is_aligned(a->q_out, 4))
-        return fail(NNE_ERR_INVALID_ARGUMENT, "f32 pointers must be 4-byte aligned");
+    for (const void *ptr : {(const void *)a->q, (const void *)a->k, (const void *)a->v, (const void *)a->q_out, (const void *)a->q_gamma,
+                            (const void *)a->k_gamma, (const void *)a->page_table, (const void *)a->sequence, (const void *)a->index,
+                            (const void *)a->position})
+        if (!is_aligned(ptr, 4)) return fail(NNE_ERR_INVALID_ARGUMENT, "device pointers must be 4-byte aligned");
     if (a->tokens == 0 || (!a->q && !a->k)) return NNE_OK;
     NNE_TRY(use_ctx(c->ctx));
     AppendArgs p = {};

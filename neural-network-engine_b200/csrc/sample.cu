@@ -805,7 +805,10 @@ extern "C" int nne_sample_dev(nne_ctx *ctx, const nne_sample *a, void *stream) {
     if (a->rows > ((size_t)1 << 27)) return fail(NNE_ERR_INVALID_ARGUMENT, "at most 2^27 rows a call, got %zu", a->rows);
     if (a->rows == 0) return NNE_OK;
     if (!a->logits || !a->uniform || !a->tokens) return fail(NNE_ERR_INVALID_ARGUMENT, "null device pointer");
-    if (reinterpret_cast<uintptr_t>(a->logits) & 3) return fail(NNE_ERR_INVALID_ARGUMENT, "logits are not 4-byte aligned");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->temperature) | reinterpret_cast<uintptr_t>(a->top_k) |
+                           reinterpret_cast<uintptr_t>(a->top_p) | reinterpret_cast<uintptr_t>(a->min_p) | reinterpret_cast<uintptr_t>(a->uniform) |
+                           reinterpret_cast<uintptr_t>(a->tokens);
+    if (bits & 3) return fail(NNE_ERR_INVALID_ARGUMENT, "device pointers must be 4-byte aligned");
     // CTAs a row: as many as leave each at least 2048 logits (four a thread), up to the 8 of a portable cluster.
     unsigned ranks = 1;
     while (ranks < 8 && a->vocab >= (size_t)ranks * 2 * 2048) ranks *= 2;

@@ -23,7 +23,9 @@ extern "C" int nne_tree_attention_dev(nne_kv_cache *c, const nne_tree_attention 
     if (!a->q || !a->out || !a->node_start || !a->context || !a->page_table)
         return fail(NNE_ERR_INVALID_ARGUMENT, "null device pointer");
     if (a->table_stride == 0) return fail(NNE_ERR_INVALID_ARGUMENT, "table_stride is 0");
-    if ((reinterpret_cast<uintptr_t>(a->q) & 3) || (reinterpret_cast<uintptr_t>(a->out) & 3) || (reinterpret_cast<uintptr_t>(a->visible) & 7))
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->node_start) |
+                           reinterpret_cast<uintptr_t>(a->context) | reinterpret_cast<uintptr_t>(a->page_table);
+    if ((bits & 3) || (reinterpret_cast<uintptr_t>(a->visible) & 7))
         return fail(NNE_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its type");
     NNE_TRY(use_ctx(c->ctx));
     TreeArgs t = {};

@@ -126,3 +126,75 @@ def test_a_prompt_and_a_drafted_tree(nne, ctx):
     verify()
     assert torch.equal(first, lg)
     ctx.check()
+
+
+def test_a_pool_beyond_32_bits(nne, ctx):
+    """Keys and values at the end of a pool of more than 2^32 elements: stored there, read from there."""
+    import torch
+    page, d, pages = 1024, 256, 16400
+    k, v = (torch.empty(pages, 1, page, d, device="cuda", dtype=torch.float16) for _ in range(2))
+    assert k.numel() > 2 ** 32
+    cache = nne.PagedKvCache(ctx, pages, page, 1, d, "f16", k.data_ptr(), v.data_ptr())
+    n = 40
+    x = torch.randn(3, n, d, device="cuda")
+    table = torch.tensor([[pages - 1]], device="cuda", dtype=torch.int32)
+    seq, at = torch.zeros(n, device="cuda", dtype=torch.int32), torch.arange(n, device="cuda", dtype=torch.int32)
+    s = torch.cuda.current_stream().cuda_stream
+    nne.KvAppend(cache, n, k=x[1].data_ptr(), v=x[2].data_ptr(), page_table=table.data_ptr(), table_stride=1, sequences=1,
+                 sequence=seq.data_ptr(), index=at.data_ptr()).run(s)
+    assert torch.equal(k[-1, 0, :n], x[1].half()) and torch.equal(v[-1, 0, :n], x[2].half())
+    out = torch.empty(n, d, device="cuda")
+    start, context = torch.tensor([0, n], device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    for rows in (n, 1):  # both kernels
+        start[1] = rows
+        nne.TreeAttention(cache, n, 1, x[0].data_ptr(), out.data_ptr(), 1, start.data_ptr(), context.data_ptr(), table.data_ptr(), 1, rows,
+                          0).run(s)
+        for r in range(rows):
+            # Scores are off by (D / 16 + 8) 2^-22 of scale * sum |q k|, which enters numerator and denominator; the probabilities'
+            # parts and the sums over one tile of keys by fewer than 40 steps of 2^-22 more.
+            keys, values, q = x[1, :r + 1].half().double(), x[2, :r + 1].half().double(), x[0, r].double()
+            w = torch.softmax(keys @ q * d ** -0.5, dim=0)
+            size = float((keys.abs() @ q.abs()).max()) * d ** -0.5
+            bound = (2 * (d / 16 + 8) * size + 40) * 2.0 ** -22 * (w @ values.abs())
+            assert bool(((out[r].double() - w @ values).abs() <= bound).all())
+
+
+FIRST_CALL = """
+import importlib, sys
+sys.path.insert(0, %r)
+import torch
+nne = importlib.import_module("neural-network-engine_b200")
+ctx = nne.default_context(0)
+k, v = (torch.randn(8, 2, 16, 64, device="cuda").half() for _ in range(2))
+q, out = torch.randn(1, 8, 64, device="cuda"), torch.zeros(1, 8, 64, device="cuda")
+i = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)
+start, context, table = i(0, 1), i(100), i(*range(8))
+cache = nne.PagedKvCache(ctx, 8, 16, 2, 64, "f16", k.data_ptr(), v.data_ptr())
+call = nne.TreeAttention(cache, 1, 8, q.data_ptr(), out.data_ptr(), 1, start.data_ptr(), context.data_ptr(), table.data_ptr(), 8, 1, 100)
+logits, u, tok = torch.randn(1, 9000, device="cuda"), torch.zeros(1, device="cuda"), i(-1)
+draw = nne.Sampler(ctx, 1, 9000, logits.data_ptr(), u.data_ptr(), tok.data_ptr())
+w, x, y = torch.randn(64, 64, device="cuda"), torch.randn(9, 64, device="cuda"), torch.zeros(9, 64, device="cuda")
+layer = nne.QLinear4.from_linear_device(ctx, w.data_ptr(), 0, 64, 64, 32)
+torch.cuda.synchronize()
+s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    call.run(s.cuda_stream)
+    draw.run(s.cuda_stream)
+    layer.forward_device(x.data_ptr(), 9, y.data_ptr(), s.cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+a, b, c = out.clone(), tok.clone(), y.clone()
+out.zero_(), tok.zero_(), y.zero_()
+call.run(), draw.run(), layer.forward_device(x.data_ptr(), 9, y.data_ptr())
+torch.cuda.synchronize()
+assert torch.equal(a, out) and torch.equal(b, tok) and torch.equal(c, y) and bool(a.any()) and bool(c.any())
+"""
+
+
+def test_a_first_call_may_be_captured(nne):
+    """In a process of its own: what the library asks the driver once is asked while a stream is being captured."""
+    import subprocess
+    import sys
+    root = oracle.ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL % root], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]

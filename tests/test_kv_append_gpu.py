@@ -217,7 +217,8 @@ def test_refusals(nne, ctx):
     c = nne.PagedKvCache(ctx, **ok, rope_dims=64)
     good = dict(tokens=2, q_heads=4, q=16, q_out=16, k=16, v=16, page_table=16, table_stride=1, sequences=1, sequence=16, index=16)
     for change in (dict(v=0), dict(q_out=0), dict(q_heads=0), dict(q_stride=100), dict(k_stride=64), dict(page_table=0), dict(index=0),
-                   dict(sequence=0), dict(table_stride=0), dict(q=18), dict(tokens=2 ** 32)):
+                   dict(sequence=0), dict(table_stride=0), dict(q=18), dict(tokens=2 ** 32), dict(index=17), dict(page_table=18), dict(q_gamma=18),
+                   dict(position=19)):
         with pytest.raises(nne.InvalidArgument):
             nne.KvAppend(c, **{**good, **change}).run()
     nne.KvAppend(c, **{**good, "tokens": 0}).run()

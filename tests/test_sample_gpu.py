@@ -187,7 +187,7 @@ def test_another_stream_and_a_captured_call(nne, ctx):
 def test_refusals(nne, ctx):
     good = dict(rows=1, vocab=10, logits=16, uniform=16, tokens=16)
     for change in (dict(vocab=0), dict(vocab=2 ** 22 + 1), dict(row_stride=9), dict(rows=2 ** 40), dict(logits=0), dict(uniform=0), dict(tokens=0),
-                   dict(logits=18)):
+                   dict(logits=18), dict(tokens=18), dict(top_k=17), dict(uniform=19)):
         with pytest.raises(nne.InvalidArgument):
             nne.Sampler(ctx, **{**good, **change}).run()
     nne.Sampler(ctx, **{**good, "rows": 0}).run()

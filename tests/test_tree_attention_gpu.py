@@ -253,7 +253,7 @@ def test_refusals(nne, ctx):
                 max_context=10)
     for change in (dict(q_heads=3), dict(q_heads=0), dict(max_nodes=65), dict(max_nodes=-1), dict(q_stride=100), dict(out_stride=64), dict(q=0),
                    dict(out=0), dict(node_start=0), dict(context=0), dict(page_table=0), dict(table_stride=0), dict(scale=float("nan")),
-                   dict(visible=12), dict(q=18), dict(tokens=2 ** 31), dict(max_context=-1), dict(sequences=-1)):
+                   dict(visible=12), dict(q=18), dict(context=18), dict(page_table=17), dict(node_start=19), dict(tokens=2 ** 31), dict(max_context=-1), dict(sequences=-1)):
         with pytest.raises(nne.InvalidArgument):
             nne.TreeAttention(c, **{**good, **change}).run()
     for change in (dict(tokens=0), dict(sequences=0), dict(max_nodes=0)):
