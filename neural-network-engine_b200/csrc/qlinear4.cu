@@ -229,6 +229,22 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Two f32 operations in one instruction, each rounded as by itself.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\n"
+        "mov.b64 {%0, %1}, d;}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -400,11 +416,12 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
     grid_dependency_wait();
     grid_launch_dependents();
 
-    float sum[TPW][NT][2], part[TPW][NT][4];
+    float2 sum[TPW][NT];  // rows r and r + 8
+    float part[TPW][NT][4];
 #pragma unroll
     for (int u = 0; u < TPW; ++u)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sum[u][t][0] = sum[u][t][1] = 0.0f;
+        for (int t = 0; t < NT; ++t) sum[u][t] = make_float2(0.0f, 0.0f);
 
     // Prepared activations of the chunks from s0 (counted in the share) on: 16-byte copies into buffer `buf`, part of
     // the copy group that is committed next.
@@ -490,14 +507,21 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
                 const bool first = pair == 0 ? (CPG == 1 || j % CPG == 0) : GPC == 2;
                 const bool last = pair == 0 ? GPC == 2 : (CPG == 1 || j % CPG == CPG - 1 || end);
                 const int grp = CPG > 1 ? j / CPG : j * GPC + (GPC == 2 ? pair : 0);
+                float2 f2[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const uint4 b = fc[(pair * NT + t) * 32];
                     if (first) {
-                        const float2 i0 = *reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4);
+                        float2 i0;
+                        if (last) {  // what the group's end needs in the same load
+                            const float4 i4 = ic[grp * S::COLS + t * 4];
+                            i0 = make_float2(i4.x, i4.y), f2[t] = make_float2(i4.z, i4.w);
+                        } else {
+                            i0 = *reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4);
+                        }
+                        const float2 i8 = mul2(i0, make_float2(16.0f, 16.0f));
 #pragma unroll
-                        for (int u = 0; u < TPW; ++u)
-                            part[u][t][0] = i0.x, part[u][t][1] = i0.y, part[u][t][2] = 16.0f * i0.x, part[u][t][3] = 16.0f * i0.y;
+                        for (int u = 0; u < TPW; ++u) part[u][t][0] = i0.x, part[u][t][1] = i0.y, part[u][t][2] = i8.x, part[u][t][3] = i8.y;
                     }
 #pragma unroll
                     for (int u = 0; u < TPW; ++u) mma_f16(part[u][t], a[u][0], b.x, b.y);
@@ -511,11 +535,11 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
                         s2[u] = reinterpret_cast<const float2 *>(slot + u * SLOT + 512)[(lane >> 2) + (GPC == 2 ? pair * 8 : 0)];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const float2 f = *(reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4) + 1);
+                        if (!first) f2[t] = *(reinterpret_cast<const float2 *>(ic + grp * S::COLS + t * 4) + 1);
 #pragma unroll
                         for (int u = 0; u < TPW; ++u) {
-                            sum[u][t][0] = fmaf(s2[u].x * f.x, fmaf(part[u][t][0], 4096.0f, part[u][t][1]), sum[u][t][0]);
-                            sum[u][t][1] = fmaf(s2[u].y * f.y, fmaf(part[u][t][2], 4096.0f, part[u][t][3]), sum[u][t][1]);
+                            const float (&d)[4] = part[u][t];
+                            sum[u][t] = fma2(mul2(s2[u], f2[t]), make_float2(fmaf(d[0], 4096.0f, d[1]), fmaf(d[2], 4096.0f, d[3])), sum[u][t]);
                         }
                     }
                 }
@@ -542,8 +566,8 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int r = (warp * TPW + u) * Q4_ROWS + (lane >> 2);
-            mysum[r * S::COLS + t * 4 + (lane & 3)] = sum[u][t][0];
-            mysum[(r + 8) * S::COLS + t * 4 + (lane & 3)] = sum[u][t][1];
+            mysum[r * S::COLS + t * 4 + (lane & 3)] = sum[u][t].x;
+            mysum[(r + 8) * S::COLS + t * 4 + (lane & 3)] = sum[u][t].y;
         }
     if (split > 1) {
         cluster_meet();
@@ -666,6 +690,7 @@ template <int GROUP>
 int launch_q4_group(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
     if (m <= 4) return launch_q4<GROUP, 1>(ql, x, m, y, ldy, s);
     if (m <= 8) return launch_q4<GROUP, 2>(ql, x, m, y, ldy, s);
+    if (m <= 12) return launch_q4<GROUP, 3>(ql, x, m, y, ldy, s);
     if (m <= 16) return launch_q4<GROUP, 4>(ql, x, m, y, ldy, s);
     return launch_q4<GROUP, 8>(ql, x, m, y, ldy, s);
 }
