@@ -14,6 +14,8 @@
 // 16 with zero codes.
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <mutex>
 #include <new>
 
 #include "common.cuh"
@@ -35,7 +37,6 @@ namespace {
 
 constexpr int Q4_ROWS = 16;        // rows of a tile
 constexpr int Q4_CHUNK = 64;       // columns of a tile
-constexpr int Q4_DEPTH = 8;        // 512-byte weight loads a warp has on their way
 constexpr int Q4_PREP = 4;         // activation pieces whose loads a warp has on their way
 constexpr int Q4_MAX_SPLIT = 8;    // CTAs of a cluster that share a row block's columns
 
@@ -216,9 +217,9 @@ dequantize4_kernel(const uint4 *__restrict__ words, const float2 *__restrict__ s
 //  At a group's end 4096 * (hi sum) + (lo sum) rounds once and joins the row's f32 sum with scale * 2^-e.  The error is
 //  that of f32 (x off by 2^-23 of its group's largest); one f16 for x would give 2^-11.
 //
-// A CTA takes 128 or 256 rows (one or two tiles a warp) and a share of the columns; the CTAs of a cluster take the shares of one
+// A CTA takes 128 or 256 rows (Q4Shape) and a share of the columns; the CTAs of a cluster take the shares of one
 // row block and add their sums up through each other's shared memory in rank order, so results do not change from
-// run to run.  Each warp streams its weights through a ring of its own, filled by asynchronous copies seven tiles ahead
+// run to run.  Each warp streams its weights through a ring of its own, filled by asynchronous copies up to seven tiles ahead
 // that start before the wait for the kernel that makes x (a layer never changes); no other warp is waited for.  (The same
 // ring in registers spilled, and a spilled load is a load waited for: 95 us instead of 47 on 8192 -> 28672, group 32.)  Up to four activation rows are put on the
 // grid by the CTAs themselves; more are put there once by a kernel before (q4_prepare_kernel): with 12 rows of
@@ -263,17 +264,19 @@ struct Q4Args {
     int vec;          // rows of x can be read as float4
 };
 
-template <int NT>
+template <int NT, int TPW>  // TPW: row tiles of a warp
 struct Q4Shape {
     static constexpr int COLS = 4 * NT;                  // activation rows of a CTA
     static constexpr int CHUNK_BYTES = 4 * NT * 256;     // fragments of 64 columns
-    // Warps of a CTA, row tiles of a warp, CTAs of an SM.  With 32 activation rows the fragments' way out of shared memory
-    // would be the limit (79 % of it busy at one tile a warp), so each serves two tiles, and a CTA has an SM to itself: 48 rows of
-    // 4096 -> 11008 79 -> 66 us.
-    static constexpr int WARPS = 8;
-    static constexpr int TPW = NT >= 8 ? 2 : 1;
-    static constexpr int PER_SM = NT >= 8 ? 1 : 2;
+    // The way out of shared memory is the limit (four rows: 58 % of it busy at one tile a warp, with 32 rows 79 %), so the
+    // fragments a warp reads serve two tiles: 8192 -> 28672, one row 30 -> 25 us, 12 rows of 4091 -> 11003 22.7 -> 20.8 us, 48 rows of
+    // 4096 -> 11008 79 -> 66 us.  One tile where two would leave SMs without a CTA.  5 to 16 rows: CTAs of four warps, whose 128 rows
+    // split a layer as finely as eight of one tile (with 256 rows 24.7 us).
+    static constexpr int WARPS = NT > 1 && NT < 8 ? 4 : 8;
+    static constexpr int PER_SM = NT >= 8 ? 1 : 2;       // CTAs of an SM
     static constexpr int TILES = WARPS * TPW;
+    static constexpr int DEPTH = NT == 1 && TPW == 2 ? 4 : 8;  // tile copies on their way: 8 KB a scheduler or more
+    static constexpr int STAGE = NT > 1 ? DEPTH : 56;          // chunks whose activations are in shared memory, whole ring rounds
     template <int GROUP>
     __host__ __device__ static constexpr int slot() {  // bytes of a tile in a ring slot: codes, scales
         return Q4_CHUNK * Q4_ROWS / 2 + (GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP) * 64;
@@ -350,7 +353,7 @@ __host__ __device__ __forceinline__ unsigned q4_groups(unsigned c) {
 
 template <int GROUP, int NT>
 __global__ void __launch_bounds__(256) q4_prepare_kernel(const Q4Args p, uint8_t *frag, float4 *info) {
-    constexpr int COLS = Q4Shape<NT>::COLS;
+    constexpr int COLS = 4 * NT, CHUNK_BYTES = 4 * NT * 256;
     grid_dependency_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -364,15 +367,15 @@ __global__ void __launch_bounds__(256) q4_prepare_kernel(const Q4Args p, uint8_t
         q4_load_piece(p.x + row * p.k, (size_t)ck * Q4_CHUNK + (lane & 15) * 4, p.k, p.vec, v);
         const bool there = ck < p.chunks;
         q4_put_piece<GROUP, NT>(v, lane, r, there,
-                                reinterpret_cast<uint32_t *>(frag + (mb * p.chunks + ck) * Q4Shape<NT>::CHUNK_BYTES),
+                                reinterpret_cast<uint32_t *>(frag + (mb * p.chunks + ck) * CHUNK_BYTES),
                                 info + (mb * p.pgroups + q4_group<GROUP>(ck, (lane & 15) * 4)) * COLS + r);
     }
 }
 
-template <int GROUP, int NT, bool READY>
-__global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) q4_forward_kernel(const Q4Args p) {
-    using S = Q4Shape<NT>;
-    constexpr int WARPS = S::WARPS, TPW = S::TPW, ROWS = S::TILES * Q4_ROWS, D = Q4_DEPTH;
+template <int GROUP, int NT, int TPW, bool READY>
+__global__ void __launch_bounds__(Q4Shape<NT, TPW>::WARPS * 32, Q4Shape<NT, TPW>::PER_SM) q4_forward_kernel(const Q4Args p) {
+    using S = Q4Shape<NT, TPW>;
+    constexpr int WARPS = S::WARPS, ROWS = S::TILES * Q4_ROWS, D = S::DEPTH;
     constexpr int GPC = GROUP >= Q4_CHUNK ? 1 : Q4_CHUNK / GROUP;   // groups of a chunk
     constexpr int CPG = GROUP >= Q4_CHUNK ? GROUP / Q4_CHUNK : 1;   // chunks of a group
     constexpr int SLOT = S::template slot<GROUP>();
@@ -592,37 +595,83 @@ __global__ void __launch_bounds__(Q4Shape<NT>::WARPS * 32, Q4Shape<NT>::PER_SM) 
         if (p.bias) v = __fadd_rn(v, p.bias[out0 + r]);
         p.y[(row0 + c) * p.ldy + out0 + r] = v;
     }
-    if (split > 1)  // nobody leaves while a peer may still read its shared memory
-        cluster_meet();
+    if (split > 1) cluster_part();
 }
 
-template <int GROUP, int NT>
+// Shared memory: the weights' rings and activations of `stage` chunks, once or twice; at the end the sums.
+template <int GROUP, int NT, int TPW>
+size_t q4_bytes(size_t stage, bool twice) {
+    using S = Q4Shape<NT, TPW>;
+    const size_t ring = (size_t)S::TILES * S::DEPTH * S::template slot<GROUP>();
+    const size_t x = stage * S::CHUNK_BYTES + q4_groups<GROUP>((unsigned)stage) * S::COLS * sizeof(float4);
+    const size_t sums = (size_t)S::TILES * Q4_ROWS * S::COLS * sizeof(float), bytes = ring + x * (twice ? 2 : 1);
+    return bytes > sums ? bytes : sums;
+}
+
+// Clusters of 1 .. Q4_MAX_SPLIT CTAs that the GPU holds at once, asked once a device.
+template <int GROUP, int NT, int TPW>
+int q4_resident(const nne_ctx *ctx, const int **resident) {
+    using S = Q4Shape<NT, TPW>;
+    constexpr bool READY = NT > 1;
+    static std::atomic<uint64_t> known{0};
+    static int table[64][Q4_MAX_SPLIT];
+    static std::mutex mu;
+    const int dev = ctx->device & 63;
+    if (!(known.load(std::memory_order_acquire) >> dev & 1)) {
+        std::lock_guard<std::mutex> lock(mu);
+        const size_t bytes = q4_bytes<GROUP, NT, TPW>(S::STAGE, READY);
+        NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT, TPW, READY>, bytes));
+        for (int c = 1; c <= Q4_MAX_SPLIT; ++c) {
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)c;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)c, 64, 1);
+            cfg.blockDim = dim3(S::WARPS * 32);
+            cfg.dynamicSmemBytes = bytes;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, q4_forward_kernel<GROUP, NT, TPW, READY>, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            table[dev][c - 1] = c == 1 && n < 1 ? 1 : n;
+        }
+        known.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    *resident = table[dev];
+    return NNE_OK;
+}
+
+template <int GROUP, int NT, int TPW>
 int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
-    using S = Q4Shape<NT>;
+    using S = Q4Shape<NT, TPW>;
     constexpr bool READY = NT > 1;
     const nne_ctx *ctx = ql->ctx;
     const size_t blocks_n = (ql->tiles + S::TILES - 1) / S::TILES;
     const size_t blocks_m = (m + S::COLS - 1) / S::COLS;
     // Split the columns over the CTAs of a cluster: a CTA's time is its chunks and, in their measure, about ten for starting,
-    // activations and the join, and CTAs run in rounds of what the GPU holds (28672 -> 8192, one row, in 320 CTAs: 54
-    // us, in 256: 31).  A share keeps eight chunks of 64.
-    const size_t slots = (size_t)ctx->sm_count * S::PER_SM, have = blocks_n * blocks_m;
+    // activations and the join, and clusters run in rounds of what the GPU holds (28672 -> 8192, one row, in 320 CTAs: 54
+    // us, in 256: 31; 4096 -> 6144 in clusters of 6, of which 45 find a place and not 49: 12.6 us, otherwise 7.4).  A share keeps
+    // eight chunks of 64.
+    const int *resident;
+    NNE_TRY((q4_resident<GROUP, NT, TPW>(ctx, &resident)));
+    const size_t have = blocks_n * blocks_m;
     size_t split = 1;
     double least = 1e300;
     for (size_t c = 1; c <= Q4_MAX_SPLIT && (c == 1 || ql->chunks >= c * 8); ++c) {
-        const double cost = (double)((have * c + slots - 1) / slots) * ((double)ql->chunks / (double)c + 10.0);
+        if (resident[c - 1] < 1) continue;
+        const size_t rounds = (have + resident[c - 1] - 1) / resident[c - 1];
+        const double cost = (double)rounds * ((double)ql->chunks / (double)c + 10.0);
         if (cost < least * 0.98) split = c, least = cost;
     }
     // shares in whole pairs of chunks, so that a group of 128 columns never lies in two
     size_t span = (ql->chunks + split - 1) / split;
     span = (span + 1) & ~(size_t)1;
     split = (ql->chunks + span - 1) / span;
-    // Activations in shared memory beside the weight rings, in stages of whole ring rounds: two buffers for prepared
-    // ones (the next stage is copied in during this one), one for those the CTA prepares.
-    const size_t ring = (size_t)S::TILES * Q4_DEPTH * S::template slot<GROUP>();
-    auto xbytes = [](size_t chunks) { return chunks * S::CHUNK_BYTES + q4_groups<GROUP>((unsigned)chunks) * S::COLS * sizeof(float4); };
-    size_t stage = READY ? Q4_DEPTH : 7 * Q4_DEPTH;
-    if (stage >= span) stage = span;
+    const size_t stage = (size_t)S::STAGE < span ? S::STAGE : span;
     Q4Args a = {};
     a.words = ql->words;
     a.scales = ql->scales;
@@ -639,10 +688,8 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
     a.span = (unsigned)span;
     a.stage = (unsigned)stage;
     a.vec = ql->k % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    size_t bytes = ring + xbytes(stage) * (READY && stage < span ? 2 : 1);
-    const size_t sums = (size_t)S::TILES * Q4_ROWS * S::COLS * sizeof(float);
-    if (bytes < sums) bytes = sums;
-    NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT, READY>, bytes));
+    const size_t bytes = q4_bytes<GROUP, NT, TPW>(stage, READY && stage < span);
+    NNE_TRY(ensure_dynamic_smem(ctx->device, q4_forward_kernel<GROUP, NT, TPW, READY>, bytes));
 
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -675,7 +722,7 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
         cfg.blockDim = dim3(S::WARPS * 32);
         cfg.dynamicSmemBytes = bytes;
         cfg.numAttrs = 2;
-        e = cudaLaunchKernelEx(&cfg, q4_forward_kernel<GROUP, NT, READY>, a);
+        e = cudaLaunchKernelEx(&cfg, q4_forward_kernel<GROUP, NT, TPW, READY>, a);
         count_launch();
     }
     if (work) cudaFreeAsync(work, s);
@@ -688,11 +735,18 @@ int launch_q4(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t
 
 template <int GROUP>
 int launch_q4_group(const nne_qlinear4 *ql, const float *x, size_t m, float *y, size_t ldy, cudaStream_t s) {
-    if (m <= 4) return launch_q4<GROUP, 1>(ql, x, m, y, ldy, s);
-    if (m <= 8) return launch_q4<GROUP, 2>(ql, x, m, y, ldy, s);
-    if (m <= 12) return launch_q4<GROUP, 3>(ql, x, m, y, ldy, s);
-    if (m <= 16) return launch_q4<GROUP, 4>(ql, x, m, y, ldy, s);
-    return launch_q4<GROUP, 8>(ql, x, m, y, ldy, s);
+    if (m <= 4) {
+        // Two tiles a warp where CTAs of 256 rows, split as far as may be, are enough for every SM (4096 -> 4096: 128; 11008 ->
+        // 4096 so 10.5 us, with one tile 8.8).
+        const size_t most = ql->chunks / 8 < 1 ? 1 : (ql->chunks / 8 < Q4_MAX_SPLIT ? ql->chunks / 8 : Q4_MAX_SPLIT);
+        const size_t rows = Q4Shape<1, 2>::TILES * Q4_ROWS;
+        if ((ql->n + rows - 1) / rows * most < (size_t)ql->ctx->sm_count) return launch_q4<GROUP, 1, 1>(ql, x, m, y, ldy, s);
+        return launch_q4<GROUP, 1, 2>(ql, x, m, y, ldy, s);
+    }
+    if (m <= 8) return launch_q4<GROUP, 2, 2>(ql, x, m, y, ldy, s);
+    if (m <= 12) return launch_q4<GROUP, 3, 2>(ql, x, m, y, ldy, s);
+    if (m <= 16) return launch_q4<GROUP, 4, 2>(ql, x, m, y, ldy, s);
+    return launch_q4<GROUP, 8, 2>(ql, x, m, y, ldy, s);
 }
 
 __global__ void __launch_bounds__(256)

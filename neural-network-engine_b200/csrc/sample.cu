@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         }
     }
     if (r.rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
-    cluster_meet();  // nobody leaves while a peer may still read its shared memory
+    cluster_part();
 }
 
 }  // namespace
