@@ -65,7 +65,8 @@ struct Shared {
     // Sets of levels 0 and 1; count's third is that of the threads' maxima.  Each its own: no meeting lies between the looks into
     // one and the first atomics on the next.
     unsigned count[3][SM_BUCKETS], low[2][SM_BUCKETS], high[2][SM_BUCKETS], all_count[SM_BUCKETS];
-    unsigned long long list[SM_LIST];
+    unsigned long long list[SM_LIST];        // rank 0's: the cluster's
+    unsigned long long aside[SM_LIST];       // this CTA's tokens for it
     unsigned listed;
     unsigned kept;
 };
@@ -93,18 +94,6 @@ __device__ __forceinline__ unsigned ask_cluster_u32(const void *p, unsigned rank
 __device__ __forceinline__ unsigned long long ask_cluster_u64(const void *p, unsigned rank) {
     const unsigned long long v = (threadIdx.x & 31) == 0 ? ld_cluster_u64(p, rank) : 0;
     return __shfl_sync(0xffffffffu, v, 0);
-}
-__device__ __forceinline__ unsigned add_cluster_u32(const void *p, unsigned rank, unsigned v) {
-    uint32_t peer;
-    unsigned old;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(peer), "r"(v) : "memory");
-    return old;
-}
-__device__ __forceinline__ void st_cluster_u64(const void *p, unsigned rank, unsigned long long v) {
-    uint32_t peer;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer), "l"(v) : "memory");
 }
 
 // A block's prefix sums of two values a thread (places 2t and 2t + 1): `v` becomes the sums up to and with each.
@@ -141,13 +130,16 @@ struct Row {
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaxf(x - top, -3.402823466e38f) * scale));
         return x == top ? 1.0f : w;
     }
-    __device__ __forceinline__ static unsigned long long units(float w) {
-        const uint32_t b = __float_as_uint(w);  // 0 <= w <= 1: 24 bits of mantissa, an exponent of at most 127
-        return ((unsigned long long)((b & 0x7fffffu) | 0x800000u) << 17) >> min(127u - (b >> 23), 63u);
+    __device__ __forceinline__ static unsigned long long units(float w) {  // 0 <= w <= 1
+        const float a = __fadd_rz(w, 8.0f);  // its bits count 2^-20s
+        const float b = __fadd_rz(w - (a - 8.0f), 0x1p-17f);  // what is left, in 2^-40s
+        return ((unsigned long long)(__float_as_uint(a) - 0x41000000u) << 20) + (__float_as_uint(b) - 0x37000000u);
     }
 
-    // f(index, logit) for every logit of the warp, and now and then for an index behind them with -inf.  One loop, whose
-    // loads alone differ (rows that are 16-byte aligned go by float4): the bodies are inlined eight times as it is.
+    // f(index, logit) for every logit of the warp, and now and then for an index behind them with -inf; always by whole warps.  One
+    // loop, whose loads alone differ (rows that are 16-byte aligned go by float4): the bodies are inlined eight times as it is.
+    // (Loads of the next eight before these are looked at cost registers, and more than they gave: 69 instead of 58 us for 64
+    // mixed rows of 128000.)
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
         const int lane = threadIdx.x & 31;
@@ -283,9 +275,8 @@ struct Row {
     __device__ __forceinline__ unsigned draw(F &&kept, float min_p, float u) {
         return locate(
             [&](unsigned i, float x) {
-                if (!kept(i, x)) return 0ull;
                 const float w = weight(x);
-                return w < min_p ? 0ull : units(w);
+                return units(kept(i, x) & !(w < min_p) ? w : 0.0f);
             },
             [&](unsigned long long sum) {
                 const double at = (double)u * (double)sum;
@@ -425,7 +416,7 @@ struct Settings {
 
 // The token (rank 0's return value), where the list holds what is needed for it, or -2 in all CTAs.  `mine`: the largest logit
 // that this thread has seen.
-__device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
+__device__ __forceinline__ int draw_from_list_body(Row &r, Settings set, float mine) {
     Shared *s = r.s;
     const float inv = __fdiv_rn(SM_PER_T, r.temperature);
     if (!(inv < 1e30f) || isinf(r.top)) return -2;  // distances need numbers to be measured in
@@ -491,17 +482,43 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
         }
         __syncthreads();
     };
-    // Tokens nearer than `edge` but not than `near` into rank 0's list, as far as it holds them; their number.
+    // Tokens nearer than `edge` but not than `near` into rank 0's list, as far as it holds them; their number.  Each CTA puts its
+    // own aside, and rank 0 fetches them all (put one by one into its list, each had waited for rank 0's counter).
     auto gather_tokens = [&](float near, float edge, auto &&in) {
+        const int lane = threadIdx.x & 31;
         r.each([&](unsigned i, float x) {
             const float d = distance(x);
-            if (d < edge && d >= near && in(d)) {
-                const unsigned slot = add_cluster_u32(&s->listed, 0, 1);
-                if (slot < SM_LIST) st_cluster_u64(&s->list[slot], 0, (unsigned long long)key_of(x) << 32 | (0xffffffffu - i));
+            const bool hit = d < edge && d >= near && in(d);
+            const unsigned hits = __ballot_sync(0xffffffffu, hit);
+            if (hits) {
+                unsigned slot = 0;
+                if (lane == 0) slot = atomicAdd(&s->listed, __popc(hits));
+                slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(hits & ((1u << lane) - 1));
+                if (hit && slot < SM_LIST) s->aside[slot] = (unsigned long long)key_of(x) << 32 | (0xffffffffu - i);
             }
         });
         cluster_meet();
-        return ask_cluster_u32(&s->listed, 0);
+        const unsigned have = (unsigned)lane < r.ranks ? ld_cluster_u32(&s->listed, lane) : 0;
+        unsigned upto = have;  // of the ranks up to and with this lane's
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            const unsigned u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        const unsigned all = __shfl_sync(0xffffffffu, upto, r.ranks - 1);
+        if (r.rank == 0 && all <= SM_LIST) {
+            for (unsigned i0 = 0; i0 < all; i0 += SM_THREADS) {
+                const unsigned i = i0 + threadIdx.x;
+                unsigned q = 0, from = 0;
+#pragma unroll
+                for (int w = 0; w < 7; ++w) {
+                    const unsigned bound = __shfl_sync(0xffffffffu, upto, w);
+                    if (w + 1 < (int)r.ranks && i >= bound) q = w + 1, from = bound;
+                }
+                if (i < all) s->list[i] = ld_cluster_u64(&s->aside[i - from], q);  // (whoever puts it in order begins with a barrier)
+            }
+        }
+        return all;
     };
     const float far = set.min_p > 0.0f ? -logf(set.min_p) * SM_PER_T + 1.0f : END;  // what is farther min_p leaves out
 
@@ -622,7 +639,7 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
                 index = 0xffffffffu - (unsigned)cut;
                 cluster_meet();  // rank 0 goes on to use the word
             }
-            return (int)r.draw([&](unsigned i, float x) { return x > edge || (x == edge && i <= index); }, set.min_p, set.u);
+            return (int)r.draw([&](unsigned i, float x) { return (x > edge) | ((x == edge) & (i <= index)); }, set.min_p, set.u);
         }
         const float edge = last < SM_FINE ? (float)(last + 1) : (float)SM_FINE + 4.0f * (float)(last + 1 - SM_FINE);
         gather_tokens(0.0f, edge, [](float) { return true; });
@@ -682,8 +699,17 @@ __device__ __noinline__ int draw_from_list(Row &r, Settings set, float mine) {
     return (int)s->found;
 }
 
+// A row of its own: one that others point to is read again from memory behind every atomic (64 mixed rows of 128000: 65 us, so 58).
+__device__ __noinline__ int draw_from_list(Row &given, Settings set, float mine) {
+    Row r = given;
+    const int token = draw_from_list_body(r, set, mine);
+    given.meeting = r.meeting, given.round = r.round;
+    return token;
+}
+
 // The token, whatever the settings leave.
-__device__ __noinline__ int draw_by_search(Row &r, uint32_t top_key, unsigned vocab, Settings set) {
+__device__ __noinline__ int draw_by_search(const Row &given, uint32_t top_key, unsigned vocab, Settings set) {
+    Row r = given;
     uint32_t cut = KEY_NONE + 1;  // kept: key > cut, or key == cut and index <= cut_index
     unsigned cut_index = 0xffffffffu;
     auto kept = [&](unsigned i, float x) {
@@ -723,7 +749,7 @@ __device__ __noinline__ int draw_by_search(Row &r, uint32_t top_key, unsigned vo
     return (int)r.draw(kept, set.min_p, set.u);
 }
 
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) {
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(const SampleArgs p) {
     __shared__ Shared sh;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -779,11 +805,12 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs p) 
         r.scale = isinf(r.top) ? 3.402823466e38f : fminf(__fdiv_rn(1.44269504088896340736f, r.temperature), 3.402823466e38f);
         token = -2;
         // (under a temperature near or at infinity -inf would get a weight there: the search asks for the key first)
-        if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(r, set, top);
+        Row at = r;
+        if (t < 1e30f && (set.k > 0 || set.top_p < 1.0f || set.min_p > 0.0f)) token = draw_from_list(at, set, top);
         if (token == -2) {
             cluster_meet();  // the buckets have been read by everybody
             for (int i = threadIdx.x; i < 2 * SM_BUCKETS; i += SM_THREADS) (&sh.mass[0][0])[i] = 0;
-            token = draw_by_search(r, top_key, p.vocab, set);
+            token = draw_by_search(at, top_key, p.vocab, set);
         }
     }
     if (r.rank == 0 && threadIdx.x == 0) p.tokens[row] = token;
