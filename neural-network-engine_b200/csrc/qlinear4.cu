@@ -269,7 +269,7 @@ struct Q4Shape {
     static constexpr int COLS = 4 * NT;                  // activation rows of a CTA
     static constexpr int CHUNK_BYTES = 4 * NT * 256;     // fragments of 64 columns
     // The way out of shared memory is the limit (four rows: 58 % of it busy at one tile a warp, with 32 rows 79 %), so the
-    // fragments a warp reads serve two tiles: 8192 -> 28672, one row 30 -> 25 us, 12 rows of 4091 -> 11003 22.7 -> 20.8 us, 48 rows of
+    // fragments a warp reads serve two tiles: 28672 -> 8192, one row 30 -> 25 us, 12 rows of 4091 -> 11003 22.7 -> 20.8 us, 48 rows of
     // 4096 -> 11008 79 -> 66 us.  One tile where two would leave SMs without a CTA.  5 to 16 rows: CTAs of four warps, whose 128 rows
     // split a layer as finely as eight of one tile (with 256 rows 24.7 us).
     static constexpr int WARPS = NT > 1 && NT < 8 ? 4 : 8;
