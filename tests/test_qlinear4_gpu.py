@@ -116,6 +116,22 @@ def test_forward(nne, ctx, n, k, m, group):
     assert np.array_equal(y, ql.forward(x))  # the order of sums is fixed
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k,m", [(4743, 4100, 3), (37901, 70, 1), (5000, 4096, 4), (701, 2050, 12), (130, 9000, 11)])
+def test_forward_of_large_layers(nne, ctx, n, k, m, group):
+    """Layers whose blocks of 256 rows are enough for every SM, the last one ragged; and twelve rows in one pass."""
+    codes, scales = quantize4_numpy(oracle.normal(717, n + k + group, (n, k), 0.0, 0.02), group)
+    bias = oracle.normal(718, n, (n,), 0.0, 0.1)
+    x = oracle.normal(719, m + k, (m, k))
+    ql = nne.QLinear4.from_fields(pack4(codes), scales, bias, k, n, group, ctx)
+    y = ql.forward(x)
+    ref, bound = exact(codes, scales, group, x, bias)
+    assert np.all(np.abs(y - ref) <= bound), float((np.abs(y - ref) / bound).max())
+    assert np.array_equal(y, ql.forward(x))
+    if m <= 4:
+        assert np.array_equal(y[:1], ql.forward(x[:1]))
+
+
 def test_wide_ranges_inside_a_row(nne, ctx):
     """Groups of very unlike size side by side, denormals and numbers near the end of f32."""
     n, k, group = 40, 256, 32
